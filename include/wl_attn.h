@@ -401,6 +401,157 @@ typedef struct wl_cache_append_io {
 
 int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* stream);
 
+/* ---- a paged latent cache and drafted trees ------------------------------------
+ * One pool of cache rows serves requests of different lengths. A page is
+ * page_size consecutive rows ("slots") of the pool; a request's block table
+ * lists its pages in position order, so position p of request b is slot
+ * block_table[b][p / page_size] * page_size + p % page_size. The pool is a
+ * wl_latent_cache / wl_index_cache of one sequence (the seq strides are not
+ * used). Speculative decoding writes every drafted token of a request behind
+ * its context (drafted node i at position ctx_len + i), scores all of them in
+ * one attention call, then keeps the accepted path:
+ *   wl_page_plan -> wl_cache_append_paged (per layer) -> wl_mla_tree_attn (per
+ *   layer) -> wl_tree_commit.
+ * No counterpart in the reference: it decodes one sequence, one token at a
+ * time, into caches of max_seq rows (glm_loader.cuh:282-307). All lengths live
+ * on the device, so a captured graph serves changing requests. A request may
+ * have 0 to 64 drafted nodes; node 0 is the token chosen last (its cache row
+ * is not committed yet), later nodes hang from earlier ones. */
+enum { WL_TREE_MAX = 64 };
+enum { WL_F32 = 0, WL_BF16 = 1 };
+
+typedef struct wl_paged_kv {
+    wl_latent_cache latent;        /* the pool: n_pages * page_size rows             */
+    int32_t        page_size;      /* rows per page: a multiple of 8                 */
+    int32_t        n_pages;        /* n_pages * page_size must stay below 2^31       */
+    const int32_t* block_table;    /* device [batch, table_stride]                   */
+    int64_t        table_stride;   /* >= max_pages                                   */
+    int32_t        max_pages;      /* entries per row of the table                   */
+} wl_paged_kv;
+
+/* Block tables and slot maps from request lengths. Request b holds n_held[b]
+ * pages for its ctx_len[b] cached tokens and appends n_new[b]. In request
+ * order, each takes the pages it lacks from the top of the free stack (page k
+ * of the call, over all requests, is free_list[n_free - 1 - k]); a request
+ * whose pages do not all fit (then neither do those of later requests that
+ * need any), or that would not fit its table row, gets none: short_out[b] is the
+ * number of pages it lacks (0 = served) and its slots are -1. Lengths below 0
+ * set the device error word; such a request gets short_out[b] = -1, no pages
+ * and no tokens. Tokens are laid out request after request: token i of
+ * request b is row cu_new[b] + i. Rows behind the last token (a padded batch)
+ * get -1. More tokens than n_tokens set the error word; the rows that fit are
+ * written. n_held_out / n_free_out may be n_held / n_free (updated in place). */
+typedef struct wl_page_plan_io {
+    int32_t batch;
+    int32_t n_tokens;              /* rows of slot / pos / seq                       */
+    int32_t page_size;
+    int32_t n_pages;               /* pages of the pool = capacity of free_list      */
+    const int32_t* ctx_len;        /* device [batch]                                 */
+    const int32_t* n_new;          /* device [batch]                                 */
+    int32_t* block_table;          /* device [batch, table_stride]: new entries written */
+    int64_t  table_stride;
+    int32_t  max_pages;
+    const int32_t* n_held;         /* device [batch]                                 */
+    int32_t* n_held_out;           /* device [batch]                                 */
+    const int32_t* free_list;      /* device [n_pages]                               */
+    const int32_t* n_free;         /* device [1]                                     */
+    int32_t* n_free_out;           /* device [1]                                     */
+    int32_t* cu_new;               /* out, device [batch + 1]                        */
+    int32_t* short_out;            /* out, device [batch]                            */
+    int32_t* slot;                 /* out, device [n_tokens] (may be NULL if n_tokens is 0) */
+    int32_t* pos;                  /* out, device [n_tokens]                         */
+    int32_t* seq;                  /* out, device [n_tokens]                         */
+} wl_page_plan_io;
+
+int wl_page_plan(const wl_page_plan_io* io, void* stream);
+
+/* Gives the pages of the requests with done[b] != 0 back: pushed on the free
+ * stack in request and position order, n_held[b] = 0, n_free updated. Pages
+ * that would overflow the stack set the error word and are dropped. */
+int wl_page_release(int32_t batch, const int32_t* done, const int32_t* block_table, int64_t table_stride,
+                    int32_t max_pages, int32_t* n_held, int32_t* free_list, int32_t n_pages, int32_t* n_free,
+                    void* stream);
+
+/* wl_cache_append into a pool: io->pos holds the tokens' slots (the slot array
+ * of wl_page_plan), io->seq is NULL and n_seq 1; rows are checked against
+ * n_slots instead of cfg->T_max, and a slot of -1 (padding, or a request
+ * without pages) is skipped without an error. */
+int wl_cache_append_paged(const wl_attn_cfg* cfg, const wl_cache_append_io* io, int32_t n_slots, void* stream);
+
+/* Absorbed-MLA attention of drafted trees: row cu_nodes[b] + i (node i of
+ * request b) attends positions [0, ctx_len[b]) and those nodes j of its own
+ * request (positions ctx_len[b] + j) that it sees: bit j of tree_mask[row], or
+ * its ancestors by `parent` (parent[row] = index of the parent within the
+ * request, -1 for a root) and itself, or, with both NULL, nodes 0..i (a chain).
+ * WL_MODE_CONSUMER narrows this to the row's own list sel_in[row] of unique
+ * positions (any order; entries that the row may not see are dropped);
+ * WL_MODE_DENSE takes every key it sees. Rows that see nothing get ctx = 0 and
+ * lse = -inf; rows of no request (behind cu_nodes[batch]) are left as they are.
+ * Keys that a row does not see never reach it, whatever their rows hold.
+ * A request whose numbers are out of range (more than 64 nodes, rows outside
+ * [0, n_nodes), ctx_len + nodes above cfg->T_max or its table), and a table
+ * entry outside the pool, set the device error word; the request's rows are
+ * left as they are, the page's keys are left out. ctx is fp32 or bf16; P enters the P.V product
+ * in bf16 (as in wl_attn_decode), its sum in fp32 before that rounding. */
+typedef struct wl_tree_attn_io {
+    int32_t batch;
+    int32_t n_nodes;               /* rows of q_abs, ctx and lse                     */
+    const int32_t*  ctx_len;       /* device [batch]                                 */
+    const int32_t*  cu_nodes;      /* device [batch + 1], ascending from 0           */
+    const uint64_t* tree_mask;     /* device [n_nodes] or NULL                       */
+    const int32_t*  parent;        /* device [n_nodes] or NULL                       */
+    wl_paged_kv kv;
+    const void* q_abs;             /* bf16 [n_nodes, n_heads, kv_lora+rope_dim]      */
+    int32_t  mode;                 /* WL_MODE_DENSE or WL_MODE_CONSUMER              */
+    int32_t  ctx_type;             /* WL_F32 or WL_BF16                              */
+    const int32_t* sel_in;         /* consumer: device [n_nodes, sel_stride]         */
+    const int32_t* sel_n_in;       /* consumer: device [n_nodes], or NULL -> sel_n   */
+    int32_t  sel_n;
+    int64_t  sel_stride;
+    void*    ctx;                  /* out: [n_nodes, n_heads, kv_lora]               */
+    float*   lse;                  /* out, optional: fp32 [n_nodes, n_heads]         */
+} wl_tree_attn_io;
+
+size_t wl_tree_attn_workspace_bytes(const wl_attn_cfg* cfg, int32_t batch, int32_t n_nodes);
+int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* Greedy verification and commit. From node 0 of each request the path goes to
+ * the lowest child c of the current node with draft[c] == target[current] (the
+ * model's choice after it), until there is none; the cache rows of the path's
+ * nodes then move to the front of the drafted rows (position ctx_len + d for
+ * the d-th node) in every layer's caches. n_accept[b] counts the path (0 for a
+ * request without nodes), path[b] lists its nodes (-1 behind them), next[b] is
+ * target[last node] (-1 without nodes), ctx_out[b] = ctx_len[b] + n_accept[b].
+ * ctx_out must not be ctx_len. `latent` and `index` are host arrays of n_layers
+ * pools that share the block table; `index` may be NULL, and an entry without
+ * keys is skipped (a layer that owns no indexer). A parent that is not an
+ * earlier node is never followed. Bad lengths or pages set the device error
+ * word; the request's (the page's) rows then stay. */
+typedef struct wl_tree_commit_io {
+    int32_t batch;
+    int32_t n_nodes;
+    const int32_t* ctx_len;        /* device [batch]                                 */
+    const int32_t* cu_nodes;       /* device [batch + 1]                             */
+    const int32_t* parent;         /* device [n_nodes]                               */
+    const int32_t* draft;          /* device [n_nodes]: the drafted tokens           */
+    const int32_t* target;         /* device [n_nodes]: the model's token after each */
+    int32_t  page_size;
+    int32_t  n_pages;
+    const int32_t* block_table;
+    int64_t  table_stride;
+    int32_t  max_pages;
+    int32_t  n_layers;             /* may be 0: the walk alone                       */
+    const wl_latent_cache* latent; /* host [n_layers]                                */
+    const wl_index_cache*  index;  /* host [n_layers] or NULL                        */
+    int32_t* n_accept;             /* out, device [batch]                            */
+    int32_t* path;                 /* out, device [batch, WL_TREE_MAX]               */
+    int32_t* next;                 /* out, device [batch]                            */
+    int32_t* ctx_out;              /* out, device [batch]                            */
+} wl_tree_commit_io;
+
+int wl_tree_commit(const wl_attn_cfg* cfg, const wl_tree_commit_io* io, void* stream);
+
 /* ---- diagnostics ------------------------------------------------------------ */
 /* Device-side error word of the calling thread's current device: bounds-check
  * failures and bounded-wait timeouts of any kernel of this library set it.
@@ -455,7 +606,8 @@ int wl_diag_xmerge(int32_t nranks, int32_t batch, int32_t nsplit, const float* o
 
 /* sizeof of each public struct, for binding checks: fills up to n entries in
  * the order cfg, latent_cache, index_cache, rows, index_share, decode_io,
- * prefill_io, shard, cache_append_io; returns how many exist. */
+ * prefill_io, shard, cache_append_io, paged_kv, page_plan_io, tree_attn_io,
+ * tree_commit_io; returns how many exist. */
 int32_t wl_struct_sizes(int64_t* out, int32_t n);
 int32_t wl_abi_version(void);
 

@@ -22,6 +22,8 @@ WL_ERR_CUDA, WL_ERR_NCCL, WL_ERR_TIMEOUT, WL_ERR_WORKSPACE = 4, 5, 6, 7
 WL_ERR_UNSUPPORTED, WL_ERR_DEVICE = 8, 9
 WL_MODE_OWNER, WL_MODE_CONSUMER, WL_MODE_DENSE = 0, 1, 2
 WL_SEL_CANONICAL = 1
+WL_TREE_MAX = 64
+WL_F32, WL_BF16 = 0, 1
 
 
 class AttnCfg(C.Structure):
@@ -75,7 +77,36 @@ class CacheAppendIO(C.Structure):
                 ("n_seq", i32)]
 
 
-STRUCTS = [AttnCfg, LatentCache, IndexCache, Rows, IndexShareC, DecodeIO, PrefillIO, Shard, CacheAppendIO]
+class PagedKVC(C.Structure):
+    _fields_ = [("latent", LatentCache), ("page_size", i32), ("n_pages", i32), ("block_table", vp),
+                ("table_stride", i64), ("max_pages", i32)]
+
+
+class PagePlanIO(C.Structure):
+    _fields_ = [("batch", i32), ("n_tokens", i32), ("page_size", i32), ("n_pages", i32), ("ctx_len", vp),
+                ("n_new", vp), ("block_table", vp), ("table_stride", i64), ("max_pages", i32),
+                ("n_held", vp), ("n_held_out", vp), ("free_list", vp), ("n_free", vp),
+                ("n_free_out", vp), ("cu_new", vp), ("short_out", vp), ("slot", vp), ("pos", vp),
+                ("seq", vp)]
+
+
+class TreeAttnIO(C.Structure):
+    _fields_ = [("batch", i32), ("n_nodes", i32), ("ctx_len", vp), ("cu_nodes", vp), ("tree_mask", vp),
+                ("parent", vp), ("kv", PagedKVC), ("q_abs", vp), ("mode", i32), ("ctx_type", i32),
+                ("sel_in", vp), ("sel_n_in", vp), ("sel_n", i32), ("sel_stride", i64), ("ctx", vp),
+                ("lse", vp)]
+
+
+class TreeCommitIO(C.Structure):
+    _fields_ = [("batch", i32), ("n_nodes", i32), ("ctx_len", vp), ("cu_nodes", vp), ("parent", vp),
+                ("draft", vp), ("target", vp), ("page_size", i32), ("n_pages", i32), ("block_table", vp),
+                ("table_stride", i64), ("max_pages", i32), ("n_layers", i32),
+                ("latent", C.POINTER(LatentCache)), ("index", C.POINTER(IndexCache)), ("n_accept", vp),
+                ("path", vp), ("next", vp), ("ctx_out", vp)]
+
+
+STRUCTS = [AttnCfg, LatentCache, IndexCache, Rows, IndexShareC, DecodeIO, PrefillIO, Shard, CacheAppendIO,
+           PagedKVC, PagePlanIO, TreeAttnIO, TreeCommitIO]
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -113,6 +144,12 @@ SIGNATURES = {
     "wl_device_error": (C.c_int, [i32, C.POINTER(u32)]),
     "wl_attn_decode_noalloc": (C.c_int, [C.POINTER(AttnCfg), C.POINTER(DecodeIO), vp]),
     "wl_cache_append": (C.c_int, [C.POINTER(AttnCfg), C.POINTER(CacheAppendIO), vp]),
+    "wl_cache_append_paged": (C.c_int, [C.POINTER(AttnCfg), C.POINTER(CacheAppendIO), i32, vp]),
+    "wl_page_plan": (C.c_int, [C.POINTER(PagePlanIO), vp]),
+    "wl_page_release": (C.c_int, [i32, vp, vp, i64, i32, vp, vp, i32, vp, vp]),
+    "wl_tree_attn_workspace_bytes": (C.c_size_t, [C.POINTER(AttnCfg), i32, i32]),
+    "wl_mla_tree_attn": (C.c_int, [C.POINTER(AttnCfg), C.POINTER(TreeAttnIO), vp, C.c_size_t, vp]),
+    "wl_tree_commit": (C.c_int, [C.POINTER(AttnCfg), C.POINTER(TreeCommitIO), vp]),
     "wl_indexer_query": (C.c_int, [C.POINTER(AttnCfg), i32, vp, i64, vp, vp, i64, i32, vp, vp, vp, vp, vp, vp]),
     "wl_mla_absorb_q": (C.c_int, [C.POINTER(AttnCfg), i32, vp, i64, vp, vp, i64, vp]),
     "wl_mla_project_v": (C.c_int, [C.POINTER(AttnCfg), i32, vp, i64, vp, vp, i64, vp]),

@@ -235,20 +235,13 @@ def mla_project_v(cfg: AttnCfg, ctx: torch.Tensor, kv_b: torch.Tensor) -> torch.
 
 # ---- the cache write path ---------------------------------------------------------------------
 
-def cache_append(cfg: AttnCfg, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
-                 keys: IndexKeys | None = None, k_raw: torch.Tensor | None = None,
-                 k_norm_w: torch.Tensor | None = None, k_norm_b: torch.Tensor | None = None,
-                 ln_eps: float = 1e-6, kv: LatentKV | None = None, kv_raw: torch.Tensor | None = None,
-                 kv_norm_w: torch.Tensor | None = None, rms_eps: float = 1e-6,
-                 seq: torch.Tensor | None = None) -> None:
-    """Write n tokens into the caches (``wl_cache_append``): the reference's
-    ``launch_indexer_key`` (src/glm_kernels.cuh:432-448; numpy
-    ``indexer_keys``, tools/ref_glm_chain.py:465-480) into ``keys`` from
-    ``k_raw`` = wk(x) [n, 128] fp32, and the latent row write of
-    ``run_attention`` (src/glm_layer_runner.cuh:544-570) into ``kv`` from
-    ``kv_raw`` = kv_a_proj_with_mqa(x) [n, 576] fp32. ``pos`` [n] int32 rows,
-    ``seq`` [n] int32 sequences (None: 0), ``cos``/``sin`` [n, 32] fp32 the
-    tokens' RoPE table rows; norm weights/bias bf16."""
+def cache_append_io(pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+                    keys: IndexKeys | None = None, k_raw: torch.Tensor | None = None,
+                    k_norm_w: torch.Tensor | None = None, k_norm_b: torch.Tensor | None = None,
+                    ln_eps: float = 1e-6, kv: LatentKV | None = None, kv_raw: torch.Tensor | None = None,
+                    kv_norm_w: torch.Tensor | None = None, rms_eps: float = 1e-6,
+                    seq: torch.Tensor | None = None) -> tuple[_lib.CacheAppendIO, list]:
+    """Fill a CacheAppendIO; returns it with the tensors it points to (keep them alive)."""
     _need(pos, torch.int32, "pos")
     _need(cos, torch.float32, "cos")
     _need(sin, torch.float32, "sin")
@@ -287,6 +280,25 @@ def cache_append(cfg: AttnCfg, pos: torch.Tensor, cos: torch.Tensor, sin: torch.
     if kv_raw is not None:
         counts.append(kv.c_kv.shape[0] if kv.c_kv.dim() == 3 else 1)
     io.n_seq = min(counts) if seq is not None else 1
+    return io, hold
+
+
+def cache_append(cfg: AttnCfg, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+                 keys: IndexKeys | None = None, k_raw: torch.Tensor | None = None,
+                 k_norm_w: torch.Tensor | None = None, k_norm_b: torch.Tensor | None = None,
+                 ln_eps: float = 1e-6, kv: LatentKV | None = None, kv_raw: torch.Tensor | None = None,
+                 kv_norm_w: torch.Tensor | None = None, rms_eps: float = 1e-6,
+                 seq: torch.Tensor | None = None) -> None:
+    """Write n tokens into the caches (``wl_cache_append``): the reference's
+    ``launch_indexer_key`` (src/glm_kernels.cuh:432-448; numpy
+    ``indexer_keys``, tools/ref_glm_chain.py:465-480) into ``keys`` from
+    ``k_raw`` = wk(x) [n, 128] fp32, and the latent row write of
+    ``run_attention`` (src/glm_layer_runner.cuh:544-570) into ``kv`` from
+    ``kv_raw`` = kv_a_proj_with_mqa(x) [n, 576] fp32. ``pos`` [n] int32 rows,
+    ``seq`` [n] int32 sequences (None: 0), ``cos``/``sin`` [n, 32] fp32 the
+    tokens' RoPE table rows; norm weights/bias bf16."""
+    io, hold = cache_append_io(pos, cos, sin, keys=keys, k_raw=k_raw, k_norm_w=k_norm_w, k_norm_b=k_norm_b,
+                               ln_eps=ln_eps, kv=kv, kv_raw=kv_raw, kv_norm_w=kv_norm_w, rms_eps=rms_eps, seq=seq)
     check(lib().wl_cache_append(C.byref(cfg), C.byref(io), _stream()), "wl_cache_append")
 
 

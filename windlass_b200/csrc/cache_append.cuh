@@ -35,6 +35,7 @@ struct AppendParams {
     const int* seq;             // [n] sequence of each token, or null (all 0)
     int n_seq;                  // sequences the caches hold (seq[i] must be below it)
     int T_max;                  // rows each sequence's caches hold
+    int skip_neg;               // a row of -1 is skipped without an error (a pool's padding)
     const float* cos;           // [n][32] the token's RoPE table row
     const float* sin;
     // indexer key (skipped when k_raw is null)
@@ -74,6 +75,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS) cache_append_kernel(AppendParam
     if (tok >= p.n) return;
     const int row = p.pos[tok];
     const int sq = p.seq ? p.seq[tok] : 0;
+    if (p.skip_neg && row == -1) return;
     if (row < 0 || row >= p.T_max || sq < 0 || sq >= p.n_seq) {
         if (lane == 0) set_error(ERRC_BOUNDS, 40);
         return;

@@ -26,7 +26,9 @@
 #include "mla_attn.cuh"
 #include "mla_attn64.cuh"
 #include "p2p.cuh"
+#include "paged.cuh"
 #include "topk.cuh"
+#include "tree_attn.cuh"
 #include "xmerge.cuh"
 #include "gemv_tc.cuh"
 
@@ -56,6 +58,9 @@ void phase_stamp(cudaStream_t st) {
 
 constexpr int kMaxSplits = 32;   // split-K CTAs per decode row (the merge takes up to 32 parts)
 constexpr int kMaxDevices = 64;
+// Plans of at most this many token rows run in one launch: the plan's one CTA
+// writes the rows itself. Larger ones write them from a second, wide launch.
+constexpr int kPlanOneLaunch = 4096;
 
 #define WL_CUDA_TRY(expr)                                           \
     do {                                                            \
@@ -939,7 +944,9 @@ int32_t wl_struct_sizes(int64_t* out, int32_t n) {
                          (int64_t)sizeof(wl_index_cache),  (int64_t)sizeof(wl_rows),
                          (int64_t)sizeof(wl_index_share),  (int64_t)sizeof(wl_attn_decode_io),
                          (int64_t)sizeof(wl_attn_prefill_io), (int64_t)sizeof(wl_shard),
-                         (int64_t)sizeof(wl_cache_append_io)};
+                         (int64_t)sizeof(wl_cache_append_io), (int64_t)sizeof(wl_paged_kv),
+                         (int64_t)sizeof(wl_page_plan_io), (int64_t)sizeof(wl_tree_attn_io),
+                         (int64_t)sizeof(wl_tree_commit_io)};
     const int32_t m = (int32_t)(sizeof(s) / sizeof(s[0]));
     for (int32_t i = 0; i < n && i < m && out; ++i) out[i] = s[i];
     return m;
@@ -1126,7 +1133,8 @@ int wl_mla_project_v(const wl_attn_cfg* cfg, int32_t n, const float* ctx, int64_
 }
 
 // ---- the cache write path -------------------------------------------------------------
-int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* stream) {
+// T_max rows per sequence; `paged`: rows are slots of a pool and -1 marks a row to skip.
+static int cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, int32_t T_max, bool paged, void* stream) {
     if (!cfg_supported(cfg)) return cfg ? WL_ERR_UNSUPPORTED : WL_ERR_ARG;
     if (!io || io->n < 0) return WL_ERR_ARG;
     if (io->n == 0) return WL_OK;
@@ -1137,7 +1145,8 @@ int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* 
     p.pos = io->pos;
     p.seq = io->seq;
     p.n_seq = io->n_seq;
-    p.T_max = cfg->T_max;
+    p.T_max = T_max;
+    p.skip_neg = paged;
     p.cos = io->cos;
     p.sin = io->sin;
     if (io->k_raw) {
@@ -1145,7 +1154,7 @@ int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* 
         if (!io->k_norm_w || !io->k_norm_b || !c.keys || !c.scale || !aligned16(io->k_raw) || !aligned16(c.keys) ||
             (c.keys_seq_stride & 15) || c.keys_seq_stride < 0 || c.scale_seq_stride < 0)
             return WL_ERR_ARG;
-        if (io->seq && (c.keys_seq_stride < (int64_t)cfg->T_max * wl::IDX_D || c.scale_seq_stride < cfg->T_max))
+        if (io->seq && (c.keys_seq_stride < (int64_t)T_max * wl::IDX_D || c.scale_seq_stride < T_max))
             return WL_ERR_ARG;
         p.k_raw = io->k_raw;
         p.k_w = static_cast<const __nv_bfloat16*>(io->k_norm_w);
@@ -1163,8 +1172,8 @@ int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* 
             c.c_kv_row_stride < wl::AT_DV || c.k_rot_row_stride < wl::AT_D - wl::AT_DV || (c.c_kv_seq_stride & 7) ||
             (c.k_rot_seq_stride & 7) || c.c_kv_seq_stride < 0 || c.k_rot_seq_stride < 0)
             return WL_ERR_ARG;
-        if (io->seq && (c.c_kv_seq_stride < (int64_t)cfg->T_max * c.c_kv_row_stride ||
-                        c.k_rot_seq_stride < (int64_t)cfg->T_max * c.k_rot_row_stride))
+        if (io->seq && (c.c_kv_seq_stride < (int64_t)T_max * c.c_kv_row_stride ||
+                        c.k_rot_seq_stride < (int64_t)T_max * c.k_rot_row_stride))
             return WL_ERR_ARG;
         p.kv_raw = io->kv_raw;
         p.kv_w = static_cast<const __nv_bfloat16*>(io->kv_norm_w);
@@ -1178,6 +1187,186 @@ int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* 
     }
     const unsigned blocks = (unsigned)ceil_div(io->n, wl::CA_WARPS);
     WL_CUDA_TRY(launch_pdl(wl::cache_append_kernel, dim3(blocks), dim3(32 * wl::CA_WARPS), 0,
+                           static_cast<cudaStream_t>(stream), p));
+    return WL_OK;
+}
+
+int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* stream) {
+    return cache_append(cfg, io, cfg ? cfg->T_max : 0, false, stream);
+}
+
+// ---- the paged cache and drafted trees -------------------------------------------------
+static int check_pages(int32_t batch, int32_t page_size, int32_t n_pages, const int32_t* table, int64_t table_stride,
+                       int32_t max_pages) {
+    if (batch < 0 || page_size <= 0 || n_pages <= 0 || (int64_t)page_size * n_pages > INT32_MAX) return WL_ERR_ARG;
+    if (!table || max_pages <= 0 || table_stride < max_pages) return WL_ERR_ARG;
+    return WL_OK;
+}
+
+static int check_pool(const wl_latent_cache& c) {
+    if (!c.c_kv || !c.k_rot || !aligned16(c.c_kv) || !aligned16(c.k_rot) || (c.c_kv_row_stride & 7) ||
+        (c.k_rot_row_stride & 7) || c.c_kv_row_stride < wl::AT_DV || c.k_rot_row_stride < wl::AT_D - wl::AT_DV)
+        return WL_ERR_ARG;
+    return WL_OK;
+}
+
+int wl_page_plan(const wl_page_plan_io* io, void* stream) {
+    if (!io || io->n_tokens < 0) return WL_ERR_ARG;
+    if (int e = check_pages(io->batch, io->page_size, io->n_pages, io->block_table, io->table_stride, io->max_pages))
+        return e;
+    if ((io->batch > 0 && (!io->ctx_len || !io->n_new || !io->n_held || !io->n_held_out || !io->short_out)) ||
+        !io->free_list || !io->n_free || !io->n_free_out || !io->cu_new || (io->n_tokens > 0 && (!io->slot || !io->pos || !io->seq)))
+        return WL_ERR_ARG;
+    wl::PlanParams p{};
+    p.batch = io->batch;
+    p.n_tokens = io->n_tokens;
+    p.page_size = io->page_size;
+    p.n_pages = io->n_pages;
+    p.ctx_len = io->ctx_len;
+    p.n_new = io->n_new;
+    p.table = io->block_table;
+    p.table_stride = io->table_stride;
+    p.max_pages = io->max_pages;
+    p.held = io->n_held;
+    p.held_out = io->n_held_out;
+    p.free_list = io->free_list;
+    p.n_free = io->n_free;
+    p.n_free_out = io->n_free_out;
+    p.cu = io->cu_new;
+    p.lack = io->short_out;
+    p.slot = io->slot;
+    p.pos = io->pos;
+    p.seq = io->seq;
+    p.own_tokens = io->n_tokens <= kPlanOneLaunch;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    WL_CUDA_TRY(launch_pdl(wl::page_plan_kernel, dim3(1), dim3(wl::PLAN_THREADS), 0, st, p));
+    if (!p.own_tokens)
+        WL_CUDA_TRY(launch_pdl(wl::plan_tokens_kernel, dim3((unsigned)ceil_div(io->n_tokens, 256)), dim3(256), 0, st, p));
+    return WL_OK;
+}
+
+int wl_page_release(int32_t batch, const int32_t* done, const int32_t* block_table, int64_t table_stride,
+                    int32_t max_pages, int32_t* n_held, int32_t* free_list, int32_t n_pages, int32_t* n_free,
+                    void* stream) {
+    if (int e = check_pages(batch, 1, n_pages, block_table, table_stride, max_pages)) return e;
+    if (batch == 0) return WL_OK;
+    if (!done || !n_held || !free_list || !n_free) return WL_ERR_ARG;
+    const wl::ReleaseParams p{batch, done, block_table, table_stride, max_pages, n_held, free_list, n_pages, n_free};
+    WL_CUDA_TRY(launch_pdl(wl::page_release_kernel, dim3(1), dim3(wl::PLAN_THREADS), 0,
+                           static_cast<cudaStream_t>(stream), p));
+    return WL_OK;
+}
+
+int wl_cache_append_paged(const wl_attn_cfg* cfg, const wl_cache_append_io* io, int32_t n_slots, void* stream) {
+    if (!io || io->seq || io->n_seq != 1 || n_slots <= 0) return WL_ERR_ARG;
+    return cache_append(cfg, io, n_slots, true, stream);
+}
+
+int wl_tree_commit(const wl_attn_cfg* cfg, const wl_tree_commit_io* io, void* stream) {
+    if (!cfg_supported(cfg)) return cfg ? WL_ERR_UNSUPPORTED : WL_ERR_ARG;
+    if (!io || io->n_nodes < 0 || io->n_layers < 0 || io->batch > 65535) return WL_ERR_ARG;
+    if (int e = check_pages(io->batch, io->page_size, io->n_pages, io->block_table, io->table_stride, io->max_pages))
+        return e;
+    if ((io->n_layers > 0 && !io->latent) ||
+        (io->batch > 0 && (!io->ctx_len || !io->cu_nodes || !io->n_accept || !io->path || !io->next || !io->ctx_out ||
+                           io->ctx_out == io->ctx_len || (io->n_nodes > 0 && (!io->parent || !io->draft || !io->target)))))
+        return WL_ERR_ARG;
+    for (int32_t l = 0; l < io->n_layers; ++l) {
+        if (int e = check_pool(io->latent[l])) return e;
+        if (io->index && io->index[l].keys && (!io->index[l].scale || !aligned16(io->index[l].keys))) return WL_ERR_ARG;
+    }
+    if (io->batch == 0) return WL_OK;
+    wl::CommitParams p{};
+    p.n_nodes = io->n_nodes;
+    p.ctx_len = io->ctx_len;
+    p.cu = io->cu_nodes;
+    p.parent = io->parent;
+    p.draft = io->draft;
+    p.target = io->target;
+    p.page_size = io->page_size;
+    p.n_pages = io->n_pages;
+    p.table = io->block_table;
+    p.table_stride = io->table_stride;
+    p.max_pages = io->max_pages;
+    p.n_accept = io->n_accept;
+    p.path = io->path;
+    p.next = io->next;
+    p.ctx_out = io->ctx_out;
+    int32_t l0 = 0;
+    do {
+        p.first = l0 == 0;
+        p.n_layers = io->n_layers - l0 < wl::COMMIT_LAYERS ? io->n_layers - l0 : wl::COMMIT_LAYERS;
+        for (int32_t l = 0; l < p.n_layers; ++l) {
+            const wl_latent_cache& c = io->latent[l0 + l];
+            wl::CommitLayer& t = p.layer[l];
+            t.c_kv = static_cast<__nv_bfloat16*>(const_cast<void*>(c.c_kv));
+            t.k_rot = static_cast<__nv_bfloat16*>(const_cast<void*>(c.k_rot));
+            t.ckv_row = c.c_kv_row_stride;
+            t.krot_row = c.k_rot_row_stride;
+            t.keys = nullptr;
+            t.scale = nullptr;
+            if (io->index && io->index[l0 + l].keys) {
+                t.keys = static_cast<uint8_t*>(const_cast<void*>(io->index[l0 + l].keys));
+                t.scale = const_cast<float*>(io->index[l0 + l].scale);
+            }
+        }
+        WL_CUDA_TRY(launch_pdl(wl::tree_commit_kernel, dim3(p.n_layers > 0 ? p.n_layers : 1, io->batch),
+                               dim3(wl::COMMIT_THREADS), 0, static_cast<cudaStream_t>(stream), p));
+        l0 += p.n_layers;
+    } while (l0 < io->n_layers);
+    return WL_OK;
+}
+
+size_t wl_tree_attn_workspace_bytes(const wl_attn_cfg* cfg, int32_t batch, int32_t n_nodes) {
+    if (!cfg || batch <= 0 || n_nodes <= 0) return 0;
+    return 256;
+}
+
+int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+    if (!cfg_supported(cfg)) return cfg ? WL_ERR_UNSUPPORTED : WL_ERR_ARG;
+    if (!io || io->n_nodes < 0) return WL_ERR_ARG;
+    const wl_paged_kv& kv = io->kv;
+    if (int e = check_pages(io->batch, kv.page_size, kv.n_pages, kv.block_table, kv.table_stride, kv.max_pages)) return e;
+    if (kv.page_size & 7) return WL_ERR_ARG;
+    if (int e = check_pool(kv.latent)) return e;
+    if (io->tree_mask && io->parent) return WL_ERR_ARG;
+    if (io->mode != WL_MODE_DENSE && io->mode != WL_MODE_CONSUMER) return WL_ERR_ARG;
+    if (io->ctx_type != WL_F32 && io->ctx_type != WL_BF16) return WL_ERR_ARG;
+    if (io->batch == 0 || io->n_nodes == 0) return WL_OK;
+    if (io->mode == WL_MODE_CONSUMER &&
+        (!io->sel_in || io->sel_stride <= 0 || (!io->sel_n_in && (io->sel_n < 0 || io->sel_n > io->sel_stride))))
+        return WL_ERR_ARG;
+    if (!io->ctx_len || !io->cu_nodes || !io->q_abs || !io->ctx || !aligned16(io->q_abs) || !aligned16(io->ctx)) return WL_ERR_ARG;
+    if (!workspace || workspace_bytes < wl_tree_attn_workspace_bytes(cfg, io->batch, io->n_nodes))
+        return WL_ERR_WORKSPACE;
+    wl::TreeParams p{};
+    p.batch = io->batch;
+    p.n_nodes = io->n_nodes;
+    p.ctx_len = io->ctx_len;
+    p.cu = io->cu_nodes;
+    p.mask = reinterpret_cast<const unsigned long long*>(io->tree_mask);
+    p.parent = io->parent;
+    p.table = kv.block_table;
+    p.table_stride = kv.table_stride;
+    p.max_pages = kv.max_pages;
+    p.page_size = kv.page_size;
+    p.n_pages = kv.n_pages;
+    p.T_max = cfg->T_max;
+    p.c_kv = static_cast<const __nv_bfloat16*>(kv.latent.c_kv);
+    p.k_rot = static_cast<const __nv_bfloat16*>(kv.latent.k_rot);
+    p.ckv_row = kv.latent.c_kv_row_stride;
+    p.krot_row = kv.latent.k_rot_row_stride;
+    p.q = static_cast<const __nv_bfloat16*>(io->q_abs);
+    p.sel = io->mode == WL_MODE_CONSUMER ? io->sel_in : nullptr;
+    p.sel_stride = io->sel_stride;
+    p.sel_n_dev = io->sel_n_in;
+    p.sel_n = io->sel_n;
+    p.scale_log2 = cfg->softmax_scale * 1.4426950408889634f;
+    p.ctx = io->ctx;
+    p.ctx_bf16 = io->ctx_type == WL_BF16;
+    p.lse = io->lse;
+    WL_CUDA_TRY(launch_pdl(wl::tree_attn_simple_kernel, dim3(io->n_nodes, 8), dim3(256), 0,
                            static_cast<cudaStream_t>(stream), p));
     return WL_OK;
 }

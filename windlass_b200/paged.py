@@ -1,0 +1,314 @@
+"""A paged latent cache and drafted trees: the serving step around speculative decoding.
+
+One pool of cache rows serves requests of different lengths: a page is ``page_size``
+consecutive rows ("slots") and a request's block table lists its pages in position
+order. A step with drafted tokens is::
+
+    plan = page_plan(ctx_len, n_new, table, n_held, free_list, n_free, page_size, n_tokens)
+    cache_append_paged(cfg, plan["slot"], cos, sin, kv=kv, kv_raw=..., ...)     # each layer
+    out = mla_tree_attn(cfg, kv, q_abs, ctx_len, plan["cu"], parent=parent)     # each layer
+    done = tree_commit(layers, ctx_len, plan["cu"], parent, draft, target)
+
+Everything that changes from step to step lives in device tensors, nothing
+synchronises, and each call runs on the current stream of its tensors' device, so a
+step can be captured into a CUDA graph. Outputs and workspaces are allocated per call
+from torch's caching allocator (two streams or two graphs never share one). The C ABI
+behind these calls is in ``include/wl_attn.h``; the reference has no counterpart (it
+decodes one sequence, one token at a time, greedily).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from ._lib import AttnCfg, IndexCache, LatentCache, PagedKVC, check, lib
+from .attn import D_QK, KV_LORA, N_HEADS, IndexKeys, LatentKV, cache_append_io
+
+TREE_MAX = _lib.WL_TREE_MAX
+_I32 = torch.int32
+
+
+def _i32(t: torch.Tensor, name: str, dev: torch.device, numel: int | None = None) -> int:
+    """Address of a contiguous int32 tensor on ``dev`` with at least ``numel`` elements."""
+    if t.dtype != _I32:
+        raise ValueError(f"{name} must be {_I32}, got {t.dtype}")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev}, got {t.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if numel is not None and t.numel() < numel:
+        raise ValueError(f"{name} must hold {numel} elements, got {t.numel()}")
+    return t.data_ptr()
+
+
+def _table(t: torch.Tensor, batch: int, dev: torch.device) -> int:
+    if t.dtype != _I32 or t.dim() != 2 or t.device != dev:
+        raise ValueError(f"block_table must be a 2-D int32 tensor on {dev}")
+    if t.shape[0] < batch or (t.shape[1] > 1 and t.stride(1) != 1) or (batch > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"block_table must have {batch} rows of consecutive entries")
+    return t.data_ptr()
+
+
+class _On:
+    """The device of a call made current (as torch's own operators do), and its stream."""
+
+    def __init__(self, dev: torch.device):
+        if dev.type != "cuda":
+            raise ValueError(f"tensors must be CUDA tensors, got {dev}")
+        self.dev = dev
+        self.back = None
+
+    def __enter__(self) -> int:
+        cur = torch.cuda.current_device()
+        if cur != self.dev.index:
+            self.back = cur
+            torch.cuda.set_device(self.dev.index)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+
+
+@dataclass
+class PagedKV:
+    """One layer's latent pool: c_kv [slots, 512] and k_rot [slots, 64] bf16 (rows of any
+    stride that keeps them 16-byte aligned), pages of ``page_size`` rows (a multiple of
+    8), ``block_table`` [batch, max_pages] int32. Slots past the last whole page are
+    not used. ``packed(kv)`` splits a [slots, 576] tensor. The views are taken when
+    the object is made; their contents, the table's included, may change freely."""
+    c_kv: torch.Tensor
+    k_rot: torch.Tensor
+    page_size: int
+    block_table: torch.Tensor
+
+    @staticmethod
+    def packed(kv: torch.Tensor, page_size: int, block_table: torch.Tensor) -> "PagedKV":
+        return PagedKV(kv[:, :KV_LORA], kv[:, KV_LORA:], page_size, block_table)
+
+    def __post_init__(self):
+        ckv, krt, t = self.c_kv, self.k_rot, self.block_table
+        if ckv.dim() != 2 or krt.dim() != 2 or ckv.shape[0] != krt.shape[0]:
+            raise ValueError("c_kv and k_rot must be [slots, 512] and [slots, 64]")
+        if ckv.shape[1] != KV_LORA or krt.shape[1] != D_QK - KV_LORA:
+            raise ValueError("c_kv and k_rot must be [slots, 512] and [slots, 64]")
+        if krt.device != ckv.device:
+            raise ValueError(f"k_rot must be on {ckv.device}, got {krt.device}")
+        self.n_pages = ckv.shape[0] // self.page_size if self.page_size > 0 else 0
+        if self.page_size <= 0 or self.page_size % 8 or self.n_pages <= 0:
+            raise ValueError("page_size must be a multiple of 8 that the pool holds at least once")
+        lat = LatentKV(ckv.unsqueeze(0), krt.unsqueeze(0)).c()
+        self._c = PagedKVC(lat, self.page_size, self.n_pages, _table(t, t.shape[0], ckv.device), t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1),
+                           t.shape[1])
+
+    def c(self) -> PagedKVC:
+        return self._c
+
+    def latent(self) -> LatentKV:
+        """The pool as a cache of one sequence."""
+        return LatentKV(self.c_kv.unsqueeze(0), self.k_rot.unsqueeze(0))
+
+
+# ---- block tables and slot maps ------------------------------------------------------------------
+
+def page_plan(ctx_len: torch.Tensor, n_new: torch.Tensor, block_table: torch.Tensor, n_held: torch.Tensor,
+              free_list: torch.Tensor, n_free: torch.Tensor, page_size: int, n_tokens: int, *,
+              in_place: bool = False) -> dict:
+    """Pages and slots for ``n_new[b]`` tokens behind ``ctx_len[b]`` cached ones
+    (``wl_page_plan``). New pages come from the top of the stack ``free_list[:n_free]`` in
+    request order and are written into ``block_table``. Returns slot, pos, seq
+    [n_tokens] (rows behind the last token: -1), cu [batch + 1], short [batch] (pages a
+    request lacks; such a request gets none, and slots of -1), n_held [batch] and
+    n_free [1] after the call: new tensors, or the given ones with ``in_place``."""
+    dev = ctx_len.device
+    B, T = ctx_len.numel(), int(n_tokens)
+    out = torch.empty(3 * T + 2 * B + 1, dtype=_I32, device=dev)
+    held_out, free_out = (n_held, n_free) if in_place else (torch.empty_like(n_held), torch.empty_like(n_free))
+    slot, pos, seq = out[:T], out[T:2 * T], out[2 * T:3 * T]
+    cu, short = out[3 * T:3 * T + B + 1], out[3 * T + B + 1:]
+    base = out.data_ptr()
+    io = _lib.PagePlanIO(B, T, page_size, free_list.numel(), _i32(ctx_len, "ctx_len", dev),
+                         _i32(n_new, "n_new", dev, B), _table(block_table, B, dev),
+                         block_table.stride(0) if B > 1 else max(block_table.shape[1], 1), block_table.shape[1],
+                         _i32(n_held, "n_held", dev, B), held_out.data_ptr(), _i32(free_list, "free_list", dev),
+                         _i32(n_free, "n_free", dev, 1), free_out.data_ptr(), base + 12 * T,
+                         base + 4 * (3 * T + B + 1), base, base + 4 * T, base + 8 * T)
+    with _On(dev) as stream:
+        check(lib().wl_page_plan(C.byref(io), stream), "wl_page_plan")
+    return dict(slot=slot, pos=pos, seq=seq, cu=cu, short=short, n_held=held_out, n_free=free_out)
+
+
+def page_release(done: torch.Tensor, block_table: torch.Tensor, n_held: torch.Tensor, free_list: torch.Tensor,
+                 n_free: torch.Tensor) -> None:
+    """Push the pages of the requests with ``done[b] != 0`` back on the free stack, in
+    place (``wl_page_release``)."""
+    dev = done.device
+    B = done.numel()
+    args = (B, _i32(done, "done", dev), _table(block_table, B, dev),
+            block_table.stride(0) if B > 1 else max(block_table.shape[1], 1), block_table.shape[1],
+            _i32(n_held, "n_held", dev, B), _i32(free_list, "free_list", dev), free_list.numel(),
+            _i32(n_free, "n_free", dev, 1))
+    with _On(dev) as stream:
+        check(lib().wl_page_release(*args, stream), "wl_page_release")
+
+
+def cache_append_paged(cfg: AttnCfg, slot: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+                       kv: PagedKV | None = None, keys: IndexKeys | None = None, **kw) -> None:
+    """``cache_append`` into pools: token i goes to row ``slot[i]`` (``page_plan``'s slots), -1
+    is skipped. ``keys`` is the owner layer's index pool (keys [slots, 128], scale
+    [slots]); the other arguments are ``cache_append``'s."""
+    pools = [t for t in (kv.c_kv if kv is not None else None, keys.keys if keys is not None else None) if t is not None]
+    if not pools:
+        raise ValueError("cache_append_paged needs kv or keys")
+    if keys is not None and keys.keys.dim() != 2:
+        raise ValueError("index pools must be [slots, 128] with scales [slots]")
+    io, hold = cache_append_io(slot, cos, sin, kv=None if kv is None else kv.latent(), keys=keys, **kw)
+    n_slots = min(t.shape[0] for t in pools)
+    with _On(pools[0].device) as stream:
+        check(lib().wl_cache_append_paged(C.byref(cfg), C.byref(io), n_slots, stream), "wl_cache_append_paged")
+
+
+# ---- attention of drafted trees ------------------------------------------------------------------
+
+def mla_tree_attn(cfg: AttnCfg, kv: PagedKV, q_abs: torch.Tensor, ctx_len: torch.Tensor, cu_nodes: torch.Tensor, *,
+                  parent: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                  sel_in: torch.Tensor | None = None, sel_n_in: torch.Tensor | None = None,
+                  out_dtype: torch.dtype = torch.float32, ctx: torch.Tensor | None = None,
+                  lse: torch.Tensor | None = None) -> dict:
+    """Absorbed-MLA attention of every request's drafted nodes (``wl_mla_tree_attn``).
+
+    q_abs bf16 [n, 64, 576]; request b's rows are ``cu_nodes[b]:cu_nodes[b + 1]`` and its
+    node i sits at position ``ctx_len[b] + i``. A row sees the context and its
+    ancestors by ``parent`` [n] (int32, index within the request, -1 for a root), or the
+    nodes of ``mask`` [n] (int64 bit masks), or nodes 0..i (neither given: a chain; one node
+    is plain decode). ``sel_in`` [n, k] int32 (with counts ``sel_n_in`` [n]) narrows each
+    row to its own list of unique positions, in any order. Returns ctx [n, 64, 512] of
+    ``out_dtype`` (float32 or bfloat16) and lse [n, 64] fp32 — the given tensors, where
+    given; rows behind the last request are not written."""
+    dev = q_abs.device
+    n, B = q_abs.shape[0], ctx_len.numel()
+    if q_abs.dtype != torch.bfloat16 or tuple(q_abs.shape[1:]) != (N_HEADS, D_QK):
+        raise ValueError("q_abs must be bf16 [n, 64, 576]")
+    if kv.c_kv.device != dev:
+        raise ValueError(f"the pool must be on {dev}, got {kv.c_kv.device}")
+    if kv.block_table.shape[0] < B:
+        raise ValueError(f"block_table must have {B} rows")
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("out_dtype must be float32 or bfloat16")
+    if parent is not None and mask is not None:
+        raise ValueError("give parent or mask, not both")
+    if sel_in is None and sel_n_in is not None:
+        raise ValueError("sel_n_in needs sel_in")
+    q_abs = q_abs.contiguous()
+    m = None
+    if mask is not None:
+        if mask.dtype != torch.int64 or mask.device != dev or not mask.is_contiguous() or mask.numel() < n:
+            raise ValueError(f"mask must be a contiguous int64 tensor of {n} elements on {dev}")
+        m = mask.data_ptr()
+    par = None if parent is None else _i32(parent, "parent", dev, n)
+    mode, sel, seln, stride, k = _lib.WL_MODE_DENSE, None, None, 0, 0
+    if sel_in is not None:
+        if sel_in.dim() != 2 or sel_in.shape[0] < n or sel_in.shape[1] < 1 or (sel_in.shape[1] > 1 and sel_in.stride(1) != 1):
+            raise ValueError(f"sel_in must be [{n}, k] with consecutive entries")
+        if sel_in.dtype != _I32 or sel_in.device != dev:
+            raise ValueError(f"sel_in must be {_I32} on {dev}")
+        mode, sel, k = _lib.WL_MODE_CONSUMER, sel_in.data_ptr(), sel_in.shape[1]
+        stride = sel_in.stride(0) if sel_in.shape[0] > 1 else k
+        seln = None if sel_n_in is None else _i32(sel_n_in, "sel_n_in", dev, n)
+    if ctx is None:
+        ctx = torch.empty(n, N_HEADS, KV_LORA, dtype=out_dtype, device=dev)
+    elif ctx.dtype != out_dtype or ctx.device != dev or not ctx.is_contiguous() or ctx.numel() != n * N_HEADS * KV_LORA:
+        raise ValueError(f"ctx must be a contiguous {out_dtype} tensor [{n}, 64, 512] on {dev}")
+    if lse is None:
+        lse = torch.empty(n, N_HEADS, dtype=torch.float32, device=dev)
+    elif lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous() or lse.numel() != n * N_HEADS:
+        raise ValueError(f"lse must be a contiguous float32 tensor [{n}, 64] on {dev}")
+    io = _lib.TreeAttnIO(B, n, _i32(ctx_len, "ctx_len", dev), _i32(cu_nodes, "cu_nodes", dev, B + 1), m, par, kv.c(),
+                         q_abs.data_ptr(), mode, _lib.WL_BF16 if out_dtype == torch.bfloat16 else _lib.WL_F32, sel, seln,
+                         k, stride, ctx.data_ptr(), lse.data_ptr())
+    L = lib()
+    ws = torch.empty(max(1, L.wl_tree_attn_workspace_bytes(C.byref(cfg), B, n)), dtype=torch.uint8, device=dev)
+    with _On(dev) as stream:
+        check(L.wl_mla_tree_attn(C.byref(cfg), C.byref(io), ws.data_ptr(), ws.numel(), stream), "wl_mla_tree_attn")
+    return dict(ctx=ctx, lse=lse)
+
+
+# ---- the commit ----------------------------------------------------------------------------------
+
+class LayerCaches:
+    """The pools that ``tree_commit`` moves rows in: ``kvs`` one ``PagedKV`` per layer, ``keys``
+    None or one ``IndexKeys`` (pools [slots, 128] / [slots]) or None per layer. All layers
+    share one block table and page size."""
+
+    def __init__(self, kvs: list[PagedKV], keys: list[IndexKeys | None] | None = None):
+        if not kvs:
+            raise ValueError("LayerCaches needs at least one layer")
+        if keys is not None and len(keys) != len(kvs):
+            raise ValueError(f"{len(kvs)} latent pools, {len(keys)} index pools")
+        first = kvs[0]
+        rows = first.c_kv.shape[0]
+        for kv in kvs:
+            if kv.page_size != first.page_size or kv.block_table.data_ptr() != first.block_table.data_ptr():
+                raise ValueError("the layers must share one block table and page size")
+            if kv.c_kv.device != first.c_kv.device:
+                raise ValueError("the layers must be on one device")
+            rows = min(rows, kv.c_kv.shape[0])
+        self.kvs, self.keys = list(kvs), None if keys is None else list(keys)
+        self._latent = (LatentCache * len(kvs))(*[kv.c().latent for kv in kvs])
+        self._index = None
+        if keys is not None:
+            self._index = (IndexCache * len(kvs))()
+            for i, k in enumerate(keys):
+                if k is None:
+                    continue
+                if k.keys.dim() != 2 or k.scale.dim() != 1 or k.keys.device != first.c_kv.device or \
+                        k.scale.device != first.c_kv.device:
+                    raise ValueError("index pools must be [slots, 128] with scales [slots], on the layers' device")
+                rows = min(rows, k.keys.shape[0], k.scale.shape[0])
+                self._index[i] = k.c()
+        self.n_pages = rows // first.page_size
+        if self.n_pages <= 0:
+            raise ValueError("a pool holds less than one page")
+
+
+def tree_commit(layers: LayerCaches, ctx_len: torch.Tensor, cu_nodes: torch.Tensor, parent: torch.Tensor,
+                draft: torch.Tensor, target: torch.Tensor, cfg: AttnCfg | None = None) -> dict:
+    """Greedy verification and commit (``wl_tree_commit``): from node 0 the path goes to the
+    lowest child whose ``draft`` token is the current node's ``target`` token; its cache
+    rows move to positions ctx_len + d in every layer. Returns n_accept [batch], path
+    [batch, 64] (-1 behind the path), next [batch] (the target of the last node) and
+    ctx_len [batch] after the commit."""
+    dev = ctx_len.device
+    B, n = ctx_len.numel(), parent.numel()
+    first = layers.kvs[0]
+    kv = first.c()
+    if first.c_kv.device != dev:
+        raise ValueError(f"ctx_len must be on {first.c_kv.device}, got {dev}")
+    if first.block_table.shape[0] < B:
+        raise ValueError(f"block_table must have {B} rows")
+    out = torch.empty((TREE_MAX + 3) * B, dtype=_I32, device=dev)
+    path, acc = out[:TREE_MAX * B].view(B, TREE_MAX), out[TREE_MAX * B:]
+    base = out.data_ptr() + 4 * TREE_MAX * B
+    io = _lib.TreeCommitIO(B, n, _i32(ctx_len, "ctx_len", dev), _i32(cu_nodes, "cu_nodes", dev, B + 1),
+                           _i32(parent, "parent", dev), _i32(draft, "draft", dev, n), _i32(target, "target", dev, n),
+                           kv.page_size, layers.n_pages, kv.block_table, kv.table_stride, kv.max_pages,
+                           len(layers.kvs), layers._latent, layers._index, base, out.data_ptr(), base + 4 * B,
+                           base + 8 * B)
+    with _On(dev) as stream:
+        check(lib().wl_tree_commit(C.byref(cfg if cfg is not None else _default_cfg()), C.byref(io), stream), "wl_tree_commit")
+    return dict(n_accept=acc[:B], path=path, next=acc[B:2 * B], ctx_len=acc[2 * B:])
+
+
+_cfg: AttnCfg | None = None
+
+
+def _default_cfg() -> AttnCfg:
+    global _cfg
+    if _cfg is None:
+        c = AttnCfg()
+        lib().wl_attn_cfg_glm52(C.byref(c), 1)
+        _cfg = c
+    return _cfg
