@@ -119,6 +119,10 @@ int ensure_attrs() {
                                      wl::GvShape<wl::GV_PROJV>::BYTES));
     WL_CUDA_TRY(cudaFuncSetAttribute(wl::gemv_tc_kernel<wl::GV_ABSQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      wl::GvShape<wl::GV_ABSQ>::BYTES));
+    WL_CUDA_TRY(cudaFuncSetAttribute(wl::tree_attn_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     wl::TaLayout<false>::BYTES));
+    WL_CUDA_TRY(cudaFuncSetAttribute(wl::tree_attn_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     wl::TaLayout<true>::BYTES));
     int sms = 0;
     WL_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     g_sm_count[dev] = sms;
@@ -1317,9 +1321,17 @@ int wl_tree_commit(const wl_attn_cfg* cfg, const wl_tree_commit_io* io, void* st
     return WL_OK;
 }
 
+// Partials a call may write: the schedule keeps to four CTA rounds of them, or
+// two per node, and no node is cut into more than TA_MAX_SPLIT runs.
+static int64_t tree_parts_max(int32_t n_nodes) {
+    const int64_t most = (int64_t)n_nodes * wl::TA_MAX_SPLIT, room = 4 * 148 > 2 * (int64_t)n_nodes ? 4 * 148 : 2 * (int64_t)n_nodes;
+    return most < room ? most : room;
+}
+
 size_t wl_tree_attn_workspace_bytes(const wl_attn_cfg* cfg, int32_t batch, int32_t n_nodes) {
     if (!cfg || batch <= 0 || n_nodes <= 0) return 0;
-    return 256;
+    const size_t parts = (size_t)tree_parts_max(n_nodes);
+    return align256(parts * wl::AT_H * wl::AT_DV * 4) + align256(parts * wl::AT_H * 4) + align256((size_t)n_nodes * 8) + 256;
 }
 
 int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* workspace, size_t workspace_bytes,
@@ -1331,6 +1343,7 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     if (kv.page_size & 7) return WL_ERR_ARG;
     if (int e = check_pool(kv.latent)) return e;
     if (io->tree_mask && io->parent) return WL_ERR_ARG;
+    if (io->batch > wl::TA_MAX_BATCH || io->n_nodes > (1 << 24)) return WL_ERR_UNSUPPORTED;
     if (io->mode != WL_MODE_DENSE && io->mode != WL_MODE_CONSUMER) return WL_ERR_ARG;
     if (io->ctx_type != WL_F32 && io->ctx_type != WL_BF16) return WL_ERR_ARG;
     if (io->batch == 0 || io->n_nodes == 0) return WL_OK;
@@ -1366,8 +1379,32 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     p.ctx = io->ctx;
     p.ctx_bf16 = io->ctx_type == WL_BF16;
     p.lse = io->lse;
-    WL_CUDA_TRY(launch_pdl(wl::tree_attn_simple_kernel, dim3(io->n_nodes, 8), dim3(256), 0,
-                           static_cast<cudaStream_t>(stream), p));
+    if (int e = ensure_attrs()) return e;
+    const int64_t parts = tree_parts_max(io->n_nodes);
+    char* ws = static_cast<char*>(align_base(workspace));
+    p.parts_max = (int)parts;
+    p.o_part = reinterpret_cast<float*>(ws);
+    ws += align256((size_t)parts * wl::AT_H * wl::AT_DV * 4);
+    p.lse_part = reinterpret_cast<float*>(ws);
+    ws += align256((size_t)parts * wl::AT_H * 4);
+    p.node_tab = reinterpret_cast<int2*>(ws);
+    p.box_rows = (kv.page_size & -kv.page_size) < wl::TA_TILE ? (kv.page_size & -kv.page_size) : wl::TA_TILE;
+    wl::TreeMaps tm{};
+    if (int e = encode_q_map(&tm.q, io->q_abs, io->n_nodes)) return e;
+    const uint64_t slots = (uint64_t)kv.n_pages * kv.page_size;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p.sel) {
+        WL_CUDA_TRY(launch_pdl(wl::tree_attn_kernel<true>, dim3(sm_count()), dim3(wl::TaLayout<true>::THREADS),
+                               wl::TaLayout<true>::BYTES, st, p, tm));
+    } else {
+        if (int e = encode_bf16_2d(&tm.ckv, kv.latent.c_kv, wl::AT_DV, slots, kv.latent.c_kv_row_stride, 64, p.box_rows)) return e;
+        if (int e = encode_bf16_2d(&tm.krot, kv.latent.k_rot, wl::AT_D - wl::AT_DV, slots, kv.latent.k_rot_row_stride, 64, p.box_rows))
+            return e;
+        WL_CUDA_TRY(launch_pdl(wl::tree_attn_kernel<false>, dim3(sm_count()), dim3(wl::TaLayout<false>::THREADS),
+                               wl::TaLayout<false>::BYTES, st, p, tm));
+    }
+    const int per = io->n_nodes < 4 ? io->n_nodes : 4;
+    WL_CUDA_TRY(launch_pdl(wl::tree_merge_kernel, dim3(wl::TM_UNITS * per), dim3(128), 0, st, p));
     return WL_OK;
 }
 
