@@ -531,14 +531,15 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
             if (!mbar_wait_fast(kfull + b, (uint32_t)(entry / TA_NBUF) & 1u, 52)) return false;
             if (g_ >= 2 && !mbar_wait_fast(sfree + s, (uint32_t)((g_ >> 1) - 1) & 1u, 53)) return false;
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t tile = sK + b * L::TILE, d = tmem + (16u << 16) + (uint32_t)(s * TA_TILE);
-#pragma unroll 1
+            if (elect_one()) {
+                const uint32_t d = tmem + (16u << 16) + (uint32_t)(s * TA_TILE);
+                const uint64_t k0 = desc_sw128(sK + b * L::TILE, 16, 1024);
+#pragma unroll
                 for (int c = 0; c < AT_CHUNKS; ++c) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_bf16_ts(d, tq + (uint32_t)(c * 32 + kk * 8), desc_sw128(tile + c * L::CHUNK + kk * 32, 16, 1024),
-                                    L::IDESC_QK, (c | kk) != 0 ? 1u : 0u);
+                    for (int kk = 0; kk < 4; ++kk)  // descriptors step in 16-byte units
+                        mma_bf16_ts(d, tq + (uint32_t)(c * 32 + kk * 8), k0 + ((c * L::CHUNK + kk * 32) >> 4), L::IDESC_QK,
+                                    (c | kk) != 0 ? 1u : 0u);
                 }
                 mma_commit(sfull + s);
             }
@@ -549,15 +550,14 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
             const int b = entry % TA_NBUF;
             if (!mbar_wait_fast(pready, (uint32_t)g_ & 1u, 54)) return false;
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t tile = sK + b * L::TILE;
+            if (elect_one()) {
+                const uint64_t p0 = desc_sw128(sP, 16, 1024), v0 = desc_sw128(sK + b * L::TILE, L::CHUNK, 1024);
 #pragma unroll
                 for (int ks = 0; ks < TA_TILE / 16; ++ks) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
-                        mma_bf16(tmem + (uint32_t)(half * 256), desc_sw128(sP + ks * 32, 16, 1024),
-                                 desc_sw128(tile + (uint32_t)(4 * half) * L::CHUNK + ks * 2048, L::CHUNK, 1024), L::IDESC_PV,
-                                 (!first || ks > 0) ? 1u : 0u);
+                        mma_bf16(tmem + (uint32_t)(half * 256), p0 + ks * 2, v0 + ((4 * half * L::CHUNK + ks * 2048) >> 4),
+                                 L::IDESC_PV, (!first || ks > 0) ? 1u : 0u);
                 }
                 mma_commit(kfree + b);
                 mma_commit(pvdone);
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
             const int4 t = items[qb];
             if (t.x < 0) break;
             if (!(ok = mbar_wait_fast(qtmem, (uint32_t)it & 1u, 56))) break;  // the query is in tensor memory
-            if (lane == 0) mbar_arrive(kfree + qb);
+            if (elect_one()) mbar_arrive(kfree + qb);
             ++e;
             const int n = t.y;
             if (n > 0) ok = issue_qk(e, gt);
