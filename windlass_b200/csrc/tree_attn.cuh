@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
             if (t.x >= 0) {
                 // The next query into tensor memory: every QK of the item before is done (its scores were read).
                 const uint32_t src0 = sK + qb * L::TILE + (uint32_t)h * 128u;
-#pragma unroll 1
+#pragma unroll 3
                 for (int k = 0; k < 9; ++k) {
                     const int e0 = 32 * k + (hi_half ? 288 : 0);
                     const uint32_t src = src0 + (uint32_t)(e0 >> 6) * L::CHUNK;
@@ -627,36 +627,60 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
                 const bool any = l_run != 0.f;  // (NaN counts: it reaches the result)
                 const float inv = any ? 1.f / l_run : 0.f;
                 const float lse = any ? (m_run + log2f(l_run)) * 0.69314718055994531f : -INFINITY;
-                const int col0 = hi_half ? 256 : 0;
                 if (!hi_half) {
                     if (out_part >= 0) p.lse_part[(long long)out_part * AT_H + h] = lse;
                     else if (p.lse) p.lse[(long long)out_row * AT_H + h] = lse;
                 }
-                const long long at = (out_part >= 0 ? (long long)out_part : (long long)out_row) * AT_H + h;
-                float* of = (out_part >= 0 ? p.o_part : static_cast<float*>(p.ctx)) + at * AT_DV + col0;
-                __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(p.ctx) + at * AT_DV + col0;
+                // A warp's 16 heads pass through its own 2 KB of P's space (P.V is done with it), 128 bytes
+                // a head at a time, so that each store instruction writes four whole 128-byte lines: an item's
+                // output takes about 2,500 cycles instead of 11,000 with every thread storing its own columns.
+                const long long at = (out_part >= 0 ? (long long)out_part : (long long)out_row) * AT_H + 16 * warp;
+                const uint32_t mine = sP + (uint32_t)h * 128u, base = sP + (uint32_t)(16 * warp) * 128u;
                 const bool narrow = out_part < 0 && p.ctx_bf16;
+                char* out = narrow ? reinterpret_cast<char*>(static_cast<__nv_bfloat16*>(p.ctx) + at * AT_DV)
+                                   : reinterpret_cast<char*>((out_part >= 0 ? p.o_part : static_cast<float*>(p.ctx)) + at * AT_DV);
+                const int row_bytes = narrow ? AT_DV * 2 : AT_DV * 4;
+                auto store = [&](int byte0) {  // the staged 16 x 128 bytes to columns from byte0 on
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = 4 * k + (lane >> 3), seg = lane & 7;
+                        const uint4 x = lds_v4(base + (uint32_t)r * 128u + (uint32_t)((seg ^ r) & 7) * 16u);
+                        *reinterpret_cast<uint4*>(out + (long long)r * row_bytes + byte0 + seg * 16) = x;
+                    }
+                    __syncwarp();
+                };
+                if (narrow) {
 #pragma unroll 1
-                for (int c = 0; c < 256; c += 32) {
-                    float ov[32];
-                    tmem_ld16x2_32<256>(tmem + lane_o + (uint32_t)c, ov);
+                    for (int c = 0; c < AT_DV; c += 64) {
+                        float ov[32];
+                        tmem_ld16x2_32<32>(tmem + lane_o + (uint32_t)c, ov);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) ov[k] = any ? ov[k] * inv : 0.f;
-                    if (narrow) {
-#pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
+                        for (int k = 0; k < 4; ++k) {
                             uint32_t w[4];
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
-                                const __nv_bfloat162 b2 = __floats2bfloat162_rn(ov[k + 2 * x], ov[k + 2 * x + 1]);
+                                const float a = ov[8 * k + 2 * x], b = ov[8 * k + 2 * x + 1];
+                                const __nv_bfloat162 b2 = __floats2bfloat162_rn(any ? a * inv : 0.f, any ? b * inv : 0.f);
                                 w[x] = *reinterpret_cast<const uint32_t*>(&b2);
                             }
-                            *reinterpret_cast<uint4*>(ob + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                            sts_v4(mine + (uint32_t)(((hi_half ? 4 : 0) + k) ^ (h & 7)) * 16u, make_uint4(w[0], w[1], w[2], w[3]));
                         }
-                    } else {
+                        store(c * 2);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < AT_DV; c += 32) {
+                        float ov[16];
+                        tmem_ld16x2_16<16>(tmem + lane_o + (uint32_t)c, ov);
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4)
-                            *reinterpret_cast<float4*>(of + c + k) = make_float4(ov[k], ov[k + 1], ov[k + 2], ov[k + 3]);
+                        for (int k = 0; k < 16; ++k) ov[k] = any ? ov[k] * inv : 0.f;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            sts_v4(mine + (uint32_t)(((hi_half ? 4 : 0) + k) ^ (h & 7)) * 16u,
+                                   make_uint4(__float_as_uint(ov[4 * k]), __float_as_uint(ov[4 * k + 1]),
+                                              __float_as_uint(ov[4 * k + 2]), __float_as_uint(ov[4 * k + 3])));
+                        store(c * 4);
                     }
                 }
                 tc_fence_before();  // these reads come before the next P.V (ordered by pready)
