@@ -156,6 +156,25 @@ __device__ __forceinline__ int tree_tiles(const TreeParams& p, const TreeSeq& s)
     return (m + TA_TILE - 1) / TA_TILE;
 }
 
+// Cost of a candidate in key tiles of one CTA; too large when its partials do not fit.
+__device__ __forceinline__ float tree_cost(const TreeParams& p, int items, int parts, int C) {
+    const float cost = (float)((items + gridDim.x - 1) / gridDim.x) * ((float)C + TA_ITEM_COST) + (float)parts * TA_PART_COST;
+    return parts <= p.parts_max ? cost : 3e38f;
+}
+// C of the warp's cheapest candidate (the fewest runs among equals).
+__device__ __forceinline__ int tree_cheapest(float best, int best_s, int longest) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float c = __shfl_xor_sync(0xffffffffu, best, o);
+        const int s = __shfl_xor_sync(0xffffffffu, best_s, o);
+        if (c < best || (c == best && s < best_s)) {
+            best = c;
+            best_s = s;
+        }
+    }
+    return max(1, (longest + best_s - 1) / best_s);
+}
+
 // Tiles per item, from the lengths: with a request's nodes cut into runs of C
 // tiles, all items run in ceil(items / CTAs) rounds of about C + TA_ITEM_COST
 // tiles each, and every partial costs a write and a read. C = ceil(longest / s)
@@ -200,27 +219,53 @@ __device__ int tree_schedule(const TreeParams& p, uint8_t* scratch, int* out) {
         for (int k = 0; k < 2; ++k) {
             const int s = k == 0 ? tid + 1 : 32 + 4 * (tid + 1);
             const int C = max(1, (longest + s - 1) / s), i = tid + 32 * k;
-            const int items = acc[i], parts = acc[TA_CANDS + i];
-            const float cost = (float)((items + gridDim.x - 1) / gridDim.x) * ((float)C + TA_ITEM_COST) +
-                               (float)parts * TA_PART_COST;
-            if (parts <= p.parts_max && cost < best) {
+            const float cost = tree_cost(p, acc[i], acc[TA_CANDS + i], C);
+            if (cost < best) {
                 best = cost;
                 best_s = s;
             }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float c = __shfl_xor_sync(0xffffffffu, best, o);
-            const int s = __shfl_xor_sync(0xffffffffu, best_s, o);
-            if (c < best || (c == best && s < best_s)) {
-                best = c;
-                best_s = s;
-            }
-        }
-        if (tid == 0) *out = max(1, (longest + best_s - 1) / best_s);
+        const int c = tree_cheapest(best, best_s, longest);
+        if (tid == 0) *out = c;
     }
     __syncthreads();
     return *out;
+}
+
+// x / c for a quotient far below 2^22, by a reciprocal and one correction.
+__device__ __forceinline__ int div_near(int x, int c, float inv) {
+    int q = (int)((float)x * inv);
+    const int r = x - q * c;
+    q += r >= c ? 1 : 0;
+    return r < 0 ? q - 1 : q;
+}
+// The same choice for at most 32 requests, one a lane, by one warp: no shared
+// memory and no block barriers, so the other roles need not wait for it.
+__device__ __forceinline__ int tree_schedule_warp(const TreeParams& p, int n, int tiles) {
+    const int lane = threadIdx.x & 31;
+    int longest = tiles;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    const int s0 = lane + 1, s1 = 32 + 4 * (lane + 1);
+    const int C0 = max(1, (longest + s0 - 1) / s0), C1 = max(1, (longest + s1 - 1) / s1);
+    const float i0 = 1.f / (float)C0, i1 = 1.f / (float)C1;
+    int items0 = 0, parts0 = 0, items1 = 0, parts1 = 0;
+    for (int b = 0; b < p.batch; ++b) {
+        const int nb = __shfl_sync(0xffffffffu, n, b), tb = __shfl_sync(0xffffffffu, tiles, b);
+        const int r0 = div_near(tb + C0 - 1, C0, i0), r1 = div_near(tb + C1 - 1, C1, i1);
+        items0 += nb * r0;
+        parts0 += r0 > 1 ? nb * r0 : 0;
+        items1 += nb * r1;
+        parts1 += r1 > 1 ? nb * r1 : 0;
+    }
+    float best = tree_cost(p, items0, parts0, C0);
+    int best_s = s0;
+    const float c1 = tree_cost(p, items1, parts1, C1);
+    if (c1 < best) {
+        best = c1;
+        best_s = s1;
+    }
+    return tree_cheapest(best, best_s, longest);
 }
 
 // Walks the requests with a warp, 32 at a time, and finds the item with a given
@@ -233,15 +278,17 @@ struct TreeWalk {
     int excl_item, excl_part;
     __device__ void load(const TreeParams& p) {
         const int b = b0 + (threadIdx.x & 31);
-        r0 = n = ctx = tiles = runs = 0;
+        r0 = n = ctx = tiles = 0;
         if (b < p.batch) {
             const TreeSeq s = tree_seq(p, b);
             r0 = s.r0;
             n = s.n;
             ctx = s.ctx;
             tiles = n > 0 ? tree_tiles<SEL>(p, s) : 0;
-            runs = (tiles + C - 1) / C;
         }
+    }
+    __device__ void count() {  // items and parts of the loaded block
+        runs = (tiles + C - 1) / C;
         const int it = n * runs, pt = runs > 1 ? it : 0;
         int si = it, sp = pt;
 #pragma unroll
@@ -257,8 +304,7 @@ struct TreeWalk {
         items = __shfl_sync(0xffffffffu, si, 31);
         parts = __shfl_sync(0xffffffffu, sp, 31);
     }
-    __device__ void start(const TreeParams& p, int C_) {
-        C = C_;
+    __device__ void start(const TreeParams& p) {
         b0 = item0 = part0 = 0;
         load(p);
     }
@@ -268,6 +314,7 @@ struct TreeWalk {
         b0 += 32;
         if (b0 >= p.batch) return false;
         load(p);
+        count();
         return true;
     }
 };
@@ -333,36 +380,39 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
         fence_mbar_init();
     }
     if (warp == L::MMA_WARP) tmem_alloc(tmem_slot, 512);
+    if (warp == 4 && lane < (SEL ? 1 : 3))
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &tm.q : lane == 1 ? &tm.ckv : &tm.krot)) : "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
     pdl_trigger();
-    const int C = tree_schedule<SEL>(p, smem, chosen);
-    if (blockIdx.x == gridDim.x - 1) {
-        // the parts of every node, for the merge
-        for (int r = tid; r < p.n_nodes; r += L::THREADS) p.node_tab[r] = make_int2(0, 0);
+    if (p.batch > 32) {
+        tree_schedule<SEL>(p, smem, chosen);
+        // the schedule's scratch becomes key tiles: order its generic accesses before TMA writes
+        fence_proxy_async_smem();
         __syncthreads();
-        if (warp == 0) {
-            TreeWalk<SEL> w;
-            w.start(p, C);
-            do {
-                if (w.runs > 1)
-                    for (int j = 0; j < w.n; ++j)
-                        p.node_tab[w.r0 + j] = make_int2(w.part0 + w.excl_part + j * w.runs, w.runs);
-            } while (w.next_block(p));
-        }
     }
-    // the schedule's scratch becomes key tiles: order its generic accesses before TMA writes
-    fence_proxy_async_smem();
-    __syncthreads();
 
     if (warp >= 4 && warp < L::MMA_WARP) {
         // ---------------- producer ----------------
         const int g = tid - 128;
         TreeWalk<SEL> walk;
-        if (warp == 4) walk.start(p, C);
+        if (warp == 4) {
+            walk.start(p);
+            walk.C = p.batch > 32 ? *chosen : tree_schedule_warp(p, walk.n, walk.tiles);
+            walk.count();
+            if (blockIdx.x == gridDim.x - 1) {  // the parts of every node, for the merge
+                for (int r = lane; r < p.n_nodes; r += 32) p.node_tab[r] = make_int2(0, 0);
+                __syncwarp();
+                TreeWalk<SEL> w = walk;
+                do {
+                    if (w.runs > 1)
+                        for (int j = 0; j < w.n; ++j) p.node_tab[w.r0 + j] = make_int2(w.part0 + w.excl_part + j * w.runs, w.runs);
+                } while (w.next_block(p));
+            }
+        }
         int e = 0;  // ring entries issued
         bool ok = true;
         // Waits for ring entry e's space; all loader threads get the same answer.
@@ -390,11 +440,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
         for (int item = blockIdx.x;; item += gridDim.x) {
             TreeItem t;
             bool more = true;
-            unsigned long long see = 0;
-            if (warp == 4) {
-                more = tree_item<SEL>(p, walk, item, t);
-                if (more) see = tree_mask_of(p, t.r0, t.n, t.node);
-            }
+            if (warp == 4) more = tree_item<SEL>(p, walk, item, t);
             if constexpr (SEL) {
                 flush();
                 if (warp == 4 && lane == 0) {
@@ -407,8 +453,6 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
                         info[4] = t.n;
                         info[5] = t.tile0 * TA_TILE;
                         info[6] = max(0, min(left, t.tiles * TA_TILE));
-                        info[7] = (int)(unsigned)see;
-                        info[8] = (int)(unsigned)(see >> 32);
                     }
                 }
             }
@@ -436,15 +480,22 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
             if constexpr (!SEL) {
                 const int R = p.box_rows, nbox = TA_TILE / R;
                 const int* table = p.table + (long long)t.b * p.table_stride;
+                // this lane's box of a tile: its page, loaded a tile ahead
+                int pos = t.tile0 * TA_TILE + lane * R, page = 0;
+                if (lane < nbox && pos < t.ctx + t.n) page = __ldg(table + pos / p.page_size);
+                const unsigned long long see = tree_mask_of(p, t.r0, t.n, t.node);
                 for (int i = 0; i < n_tiles; ++i, ++e) {
                     const int pos0 = (t.tile0 + i) * TA_TILE, bb = e % TA_NBUF;
-                    // this lane's box: first slot, -1 past the request's rows or outside the pool
+                    // its first slot, -1 past the request's rows or outside the pool
                     int slot = -1;
                     bool bad = false;
-                    if (lane < nbox && pos0 + lane * R < t.ctx + t.n) {
-                        slot = page_slot(table, p.page_size, p.n_pages, pos0 + lane * R, 46);
-                        bad = slot < 0;
+                    if (lane < nbox && pos < t.ctx + t.n) {
+                        bad = page < 0 || page >= p.n_pages;
+                        if (bad) set_error(ERRC_BOUNDS, 46);
+                        else slot = page * p.page_size + pos % p.page_size;
                     }
+                    pos += TA_TILE;
+                    if (lane < nbox && pos < t.ctx + t.n && i + 1 < n_tiles) page = __ldg(table + pos / p.page_size);
                     const int have = __popc(__ballot_sync(0xffffffffu, slot >= 0));
                     const unsigned lost = __ballot_sync(0xffffffffu, bad);
                     if (!(ok = acquire())) break;
@@ -469,11 +520,18 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
                 }
             } else {
                 const int qb = info[1], ctx = info[3], n = info[4];
-                const unsigned long long mine = (unsigned)info[7] | ((unsigned long long)(unsigned)info[8] << 32);
+                if (warp == 4) {
+                    const unsigned long long see = tree_mask_of(p, t.r0, t.n, t.node);
+                    if (lane == 0) {
+                        info[7] = (int)(unsigned)see;
+                        info[8] = (int)(unsigned)(see >> 32);
+                    }
+                }
                 const int* list = p.sel + (long long)row * p.sel_stride + info[5];
                 const int* table = p.table + (long long)qb * p.table_stride;
                 // the slot of this thread's key of tile i (threads 0-63), -1 when the row does not see it
-                asm volatile("bar.sync 2, %0;" ::"n"(L::LOADERS) : "memory");  // info[] is rewritten by the next item
+                asm volatile("bar.sync 2, %0;" ::"n"(L::LOADERS) : "memory");  // info[0..6] is read, info[7..8] written
+                const unsigned long long mine = (unsigned)info[7] | ((unsigned long long)(unsigned)info[8] << 32);
                 auto slot_of = [&](int i) -> int {
                     const int k = i * TA_TILE + g;
                     if (g >= TA_TILE || k >= n_keys) return -1;
@@ -795,6 +853,15 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
         for (unsigned cut = __ballot_sync(0xffffffffu, mine.y > 1); cut; cut &= cut - 1) {
             const int l = __ffs(cut) - 1, r = r0 + l * step;
             const int part0 = __shfl_sync(0xffffffffu, mine.x, l), n = __shfl_sync(0xffffffffu, mine.y, l);
+            // the first round of partials is under way while the weights are worked out
+            const float* src = p.o_part + ((long long)part0 * AT_H + h) * AT_DV + q * 128 + lane * 4;
+            float4 v[8];
+            auto fetch = [&](int s0) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (s0 + 4 * k < n) v[k] = *reinterpret_cast<const float4*>(src + (long long)(s0 + 4 * k) * (AT_H * AT_DV));
+            };
+            fetch(wi);
             float ls[TA_MAX_SPLIT / 32], M = -INFINITY, W = 0.f;
 #pragma unroll
             for (int k = 0; k < TA_MAX_SPLIT / 32; ++k) {
@@ -817,19 +884,13 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
                     if (lane + 32 * k < n) w_sh[lane + 32 * k] = ls[k] * inv;
             }
             __syncthreads();
-            const float* src = p.o_part + ((long long)part0 * AT_H + h) * AT_DV + q * 128 + lane * 4;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int s0 = wi; s0 < n; s0 += 32) {
-                float4 v[8];
+                if (s0 > wi) fetch(s0);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int s = s0 + 4 * k;
-                    v[k] = s < n ? *reinterpret_cast<const float4*>(src + (long long)s * (AT_H * AT_DV)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int s = s0 + 4 * k;
-                    const float w = s < n ? w_sh[s] : 0.f;
+                    if (s0 + 4 * k >= n) continue;
+                    const float w = w_sh[s0 + 4 * k];
                     acc.x = fmaf(w, v[k].x, acc.x);
                     acc.y = fmaf(w, v[k].y, acc.y);
                     acc.z = fmaf(w, v[k].z, acc.z);

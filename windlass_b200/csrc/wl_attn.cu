@@ -1403,7 +1403,7 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
         WL_CUDA_TRY(launch_pdl(wl::tree_attn_kernel<false>, dim3(sm_count()), dim3(wl::TaLayout<false>::THREADS),
                                wl::TaLayout<false>::BYTES, st, p, tm));
     }
-    const int per = io->n_nodes < 4 ? io->n_nodes : 4;
+    const int per = io->n_nodes < 9 ? io->n_nodes : 9;  // 9 x 256 blocks of 4 warps: one wave
     WL_CUDA_TRY(launch_pdl(wl::tree_merge_kernel, dim3(wl::TM_UNITS * per), dim3(128), 0, st, p));
     return WL_OK;
 }
