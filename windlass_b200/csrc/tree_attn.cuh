@@ -17,10 +17,14 @@
 // HBM once and by its other nodes from L2.
 //
 // Pipeline of a CTA (mbarriers between the roles; a ring of three 72 KB tiles):
-//   producer  the item's query (one ring entry), then its key tiles. Dense: one
+//   loaders   the item's query (one ring entry), then its key tiles. Dense: one
 //             warp issues TMA boxes, one per page part and 64 columns, so the
-//             128B-swizzled tile needs no threads. Lists: 8 warps gather rows
-//             with 16-byte cp.async, two tiles in flight.
+//             128B-swizzled tile needs no threads. Lists: 8 warps gather rows with
+//             16-byte cp.async, two tiles in flight (TMA gather4 of four rows x 64
+//             columns took twice as long a tile). A tile comes and goes in two
+//             halves (columns 0-255 and the roped ones; columns 256-511): QK
+//             starts on the first while the second is on its way, and P.V gives
+//             the first back while it reads the second.
 //   MMA       QK of tile i + 1 (A = the query in tensor memory), then P.V of
 //             tile i: the softmax of tile i runs under QK of tile i + 1.
 //   softmax   4 warps, two threads a head: query into tensor memory, mask,
@@ -114,16 +118,17 @@ __device__ __forceinline__ unsigned long long tree_mask_of(const TreeParams& p, 
 
 constexpr int TA_TILE = 64;
 constexpr int TA_NBUF = 3;
-constexpr int TA_GATHER_WARPS = 8;
+constexpr int TA_LOAD_WARP = 4;       // warps 0-3 softmax, then the loaders (dense 1 warp, lists 8), then MMA
+constexpr int TA_SCHED_THREADS = 192;
 constexpr int TA_MAX_BATCH = 16384;   // the schedule's table of a CTA (8 bytes a request) fits the key tiles' space
-constexpr int TA_CANDS = 64;          // candidate splits: 1..32, then 36, 40, .. 160
+constexpr int TA_CANDS = 64;          // candidate splits: 1..32, then 36, 40, .. 160 (3 x TA_CANDS threads sum up)
 constexpr int TA_MAX_SPLIT = 160;
 constexpr float TA_ITEM_COST = 3.f;   // an item's fixed cost (query in, output out, pipeline fill), in key tiles
 constexpr float TA_PART_COST = 0.04f; // a partial written and joined, in key tiles of one CTA
 
 template <bool SEL>
 struct TaLayout {
-    static constexpr int LOADERS = SEL ? 32 * TA_GATHER_WARPS : 32;
+    static constexpr int LOADERS = SEL ? 256 : 32;
     static constexpr int THREADS = 128 + LOADERS + 32;
     static constexpr int MMA_WARP = (128 + LOADERS) / 32;
     static constexpr uint32_t CHUNK = TA_TILE * 128;
@@ -131,16 +136,16 @@ struct TaLayout {
     static constexpr uint32_t OFF_P = TA_NBUF * TILE;
     static constexpr uint32_t OFF_ITEM = OFF_P + AT_H * 128;           // int4 per ring entry
     static constexpr uint32_t OFF_SEE = OFF_ITEM + TA_NBUF * 16;       // valid-key bits per ring entry
-    static constexpr uint32_t OFF_ROWS = OFF_SEE + TA_NBUF * 8 + 8;    // gathered rows (lists only)
+    static constexpr uint32_t OFF_ROWS = OFF_SEE + TA_NBUF * 8 + 8;    // gathered slots (lists only)
     static constexpr uint32_t OFF_BAR = OFF_ROWS + (SEL ? TA_NBUF * TA_TILE * 4 : 0);
-    static constexpr int N_BARS = 2 * TA_NBUF + 4 + 3;  // kfull, kfree, sfull[2], sfree[2], pready, pvdone, qtmem
-    static constexpr uint32_t OFF_MISC = OFF_BAR + N_BARS * 8;         // tensor-memory slot, go flag, chosen C, node info
+    static constexpr int N_BARS = 4 * TA_NBUF + 2 + 3;  // kfull[3][2], kfree[3][2], sfull[2], pready, pvdone, qtmem
+    static constexpr uint32_t OFF_MISC = OFF_BAR + N_BARS * 8;         // tensor-memory slot, longest request, go flags, item
     static constexpr uint32_t BYTES = OFF_MISC + 64 + 1024;
     static constexpr uint32_t IDESC_QK = idesc_bf16(64, TA_TILE, 0, 0);
     static constexpr uint32_t IDESC_PV = idesc_bf16(64, 256, 0, 1);
 };
 static_assert(TaLayout<true>::BYTES <= 232448 && TaLayout<false>::BYTES <= 232448, "one CTA per SM");
-static_assert(TA_MAX_BATCH * 8 + 1024 <= TA_NBUF * 73728, "schedule table");
+static_assert(TA_MAX_BATCH * 8 <= TaLayout<false>::OFF_P, "schedule table");
 
 // Keys of a row's list (clamped to the list's room).
 __device__ __forceinline__ int tree_list_n(const TreeParams& p, int r) {
@@ -156,82 +161,6 @@ __device__ __forceinline__ int tree_tiles(const TreeParams& p, const TreeSeq& s)
     return (m + TA_TILE - 1) / TA_TILE;
 }
 
-// Cost of a candidate in key tiles of one CTA; too large when its partials do not fit.
-__device__ __forceinline__ float tree_cost(const TreeParams& p, int items, int parts, int C) {
-    const float cost = (float)((items + gridDim.x - 1) / gridDim.x) * ((float)C + TA_ITEM_COST) + (float)parts * TA_PART_COST;
-    return parts <= p.parts_max ? cost : 3e38f;
-}
-// C of the warp's cheapest candidate (the fewest runs among equals).
-__device__ __forceinline__ int tree_cheapest(float best, int best_s, int longest) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float c = __shfl_xor_sync(0xffffffffu, best, o);
-        const int s = __shfl_xor_sync(0xffffffffu, best_s, o);
-        if (c < best || (c == best && s < best_s)) {
-            best = c;
-            best_s = s;
-        }
-    }
-    return max(1, (longest + best_s - 1) / best_s);
-}
-
-// Tiles per item, from the lengths: with a request's nodes cut into runs of C
-// tiles, all items run in ceil(items / CTAs) rounds of about C + TA_ITEM_COST
-// tiles each, and every partial costs a write and a read. C = ceil(longest / s)
-// for 64 values of s; the cheapest that fits the workspace is taken, the fewest
-// parts among equals. Every CTA computes the same choice (no launch of its own).
-template <bool SEL>
-__device__ int tree_schedule(const TreeParams& p, uint8_t* scratch, int* out) {
-    int* acc = reinterpret_cast<int*>(scratch);  // [64] items, [64] parts, longest
-    int2* tab = reinterpret_cast<int2*>(scratch + 1024);
-    const int tid = threadIdx.x, nthr = TaLayout<SEL>::THREADS;
-    for (int i = tid; i < 2 * TA_CANDS + 1; i += nthr) acc[i] = 0;
-    __syncthreads();
-    int longest = 0;
-    for (int b = tid; b < p.batch; b += nthr) {
-        const TreeSeq s = tree_seq(p, b);
-        const int t = s.n > 0 ? tree_tiles<SEL>(p, s) : 0;
-        tab[b] = make_int2(s.n, t);
-        longest = max(longest, t);
-    }
-    if (longest > 0) atomicMax(acc + 2 * TA_CANDS, longest);
-    __syncthreads();
-    longest = acc[2 * TA_CANDS];
-    const int cand = tid % TA_CANDS, grp = tid / TA_CANDS, ngrp = nthr / TA_CANDS;
-    if (grp < ngrp && longest > 0) {
-        const int s = cand < 32 ? cand + 1 : 32 + 4 * (cand - 31);
-        const int C = (longest + s - 1) / s;
-        int items = 0, parts = 0;
-        for (int b = grp; b < p.batch; b += ngrp) {
-            const int2 v = tab[b];
-            const int runs = (v.y + C - 1) / C;
-            items += v.x * runs;
-            parts += runs > 1 ? v.x * runs : 0;
-        }
-        atomicAdd(acc + cand, items);
-        atomicAdd(acc + TA_CANDS + cand, parts);
-    }
-    __syncthreads();
-    if (tid < 32) {
-        float best = 3e38f;
-        int best_s = 1;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int s = k == 0 ? tid + 1 : 32 + 4 * (tid + 1);
-            const int C = max(1, (longest + s - 1) / s), i = tid + 32 * k;
-            const float cost = tree_cost(p, acc[i], acc[TA_CANDS + i], C);
-            if (cost < best) {
-                best = cost;
-                best_s = s;
-            }
-        }
-        const int c = tree_cheapest(best, best_s, longest);
-        if (tid == 0) *out = c;
-    }
-    __syncthreads();
-    return *out;
-}
-
 // x / c for a quotient far below 2^22, by a reciprocal and one correction.
 __device__ __forceinline__ int div_near(int x, int c, float inv) {
     int q = (int)((float)x * inv);
@@ -239,56 +168,132 @@ __device__ __forceinline__ int div_near(int x, int c, float inv) {
     q += r >= c ? 1 : 0;
     return r < 0 ? q - 1 : q;
 }
-// The same choice for at most 32 requests, one a lane, by one warp: no shared
-// memory and no block barriers, so the other roles need not wait for it.
-__device__ __forceinline__ int tree_schedule_warp(const TreeParams& p, int n, int tiles) {
+
+// Tiles per item, from the lengths: a request's nodes are cut into the fewest
+// equal runs of at most C tiles, with C = ceil(longest / s) for 64 values of s.
+// The CTAs take the items in order, forth and back (item_of); with the longest
+// requests first (up to 32 requests are sorted) full rounds balance out, so a
+// choice costs the mean of its full rounds plus the longest item of the last one,
+// plus a write and a read per partial: within 5 % of the best of all choices on
+// 26 drawn workloads. The cheapest that fits the workspace is taken, the fewest
+// runs among equals. Every CTA computes the same choice, all its threads sharing
+// the sums (64 candidates x 3 thirds of the requests); the producer warp, which
+// alone needs it, ends with C. tab: (nodes, tiles) of each request; acc: 4 x 3 x 64.
+struct TreeCost {
+    int items[3][TA_CANDS], parts[3][TA_CANDS];
+    float sum[3][TA_CANDS], last[3][TA_CANDS];
+};
+__device__ __forceinline__ int tree_candidate(int c) { return c < 32 ? c + 1 : 32 + 4 * (c - 31); }
+
+__device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* tab, int longest, TreeCost* acc) {
+    const int cand = threadIdx.x % TA_CANDS, grp = threadIdx.x / TA_CANDS, G = gridDim.x;
+    const int per = (p.batch + 2) / 3, b0 = min(grp * per, p.batch), b1 = min(b0 + per, p.batch);
+    const int s = tree_candidate(cand), C = max(1, (longest + s - 1) / s);
+    const float inv = 1.f / (float)C;
+    const bool mine = threadIdx.x < TA_SCHED_THREADS;
+    if (mine) {
+        int items = 0, parts = 0;
+#pragma unroll 1
+        for (int b = b0; b < b1; ++b) {
+            const int2 v = tab[b];
+            const int r = div_near(v.y + C - 1, C, inv);
+            items += v.x * r;
+            parts += r > 1 ? v.x * r : 0;
+        }
+        acc->items[grp][cand] = items;
+        acc->parts[grp][cand] = parts;
+    }
+    __syncthreads();
+    if (mine) {
+        const int all = acc->items[0][cand] + acc->items[1][cand] + acc->items[2][cand], full = all / G * G;
+        int seen = (grp > 0 ? acc->items[0][cand] : 0) + (grp > 1 ? acc->items[1][cand] : 0);
+        float sum = 0.f, last = 0.f;
+#pragma unroll 1
+        for (int b = b0; b < b1; ++b) {
+            const int2 v = tab[b];
+            const int r = div_near(v.y + C - 1, C, inv), it = v.x * r;
+            if (it == 0) continue;
+            const float len = __fdividef((float)v.y, (float)r) + TA_ITEM_COST;
+            sum += (float)max(0, min(it, full - seen)) * len;
+            seen += it;
+            if (seen > full) last = fmaxf(last, len);
+        }
+        acc->sum[grp][cand] = sum;
+        acc->last[grp][cand] = last;
+    }
+    __syncthreads();
+    if (threadIdx.x / 32 != TA_LOAD_WARP) return 0;
     const int lane = threadIdx.x & 31;
-    int longest = tiles;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-    const int s0 = lane + 1, s1 = 32 + 4 * (lane + 1);
-    const int C0 = max(1, (longest + s0 - 1) / s0), C1 = max(1, (longest + s1 - 1) / s1);
-    const float i0 = 1.f / (float)C0, i1 = 1.f / (float)C1;
-    int items0 = 0, parts0 = 0, items1 = 0, parts1 = 0;
-    for (int b = 0; b < p.batch; ++b) {
-        const int nb = __shfl_sync(0xffffffffu, n, b), tb = __shfl_sync(0xffffffffu, tiles, b);
-        const int r0 = div_near(tb + C0 - 1, C0, i0), r1 = div_near(tb + C1 - 1, C1, i1);
-        items0 += nb * r0;
-        parts0 += r0 > 1 ? nb * r0 : 0;
-        items1 += nb * r1;
-        parts1 += r1 > 1 ? nb * r1 : 0;
+    float best = 3e38f;
+    int best_s = 1;
+#pragma unroll 1
+    for (int c = lane; c < TA_CANDS; c += 32) {
+        const int n_parts = acc->parts[0][c] + acc->parts[1][c] + acc->parts[2][c];
+        const float cost = (acc->sum[0][c] + acc->sum[1][c] + acc->sum[2][c]) / (float)G +
+                           fmaxf(fmaxf(acc->last[0][c], acc->last[1][c]), acc->last[2][c]) + (float)n_parts * TA_PART_COST;
+        if (n_parts <= p.parts_max && cost < best) {
+            best = cost;
+            best_s = tree_candidate(c);
+        }
     }
-    float best = tree_cost(p, items0, parts0, C0);
-    int best_s = s0;
-    const float c1 = tree_cost(p, items1, parts1, C1);
-    if (c1 < best) {
-        best = c1;
-        best_s = s1;
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) {
+        const float c = __shfl_xor_sync(0xffffffffu, best, o);
+        const int t = __shfl_xor_sync(0xffffffffu, best_s, o);
+        if (c < best || (c == best && t < best_s)) {
+            best = c;
+            best_s = t;
+        }
     }
-    return tree_cheapest(best, best_s, longest);
+    return max(1, (longest + best_s - 1) / best_s);
 }
+// A CTA's item of round k: the CTAs take them forth and back.
+__device__ __forceinline__ int item_of(int k) {
+    return k * (int)gridDim.x + ((k & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+}
+
 
 // Walks the requests with a warp, 32 at a time, and finds the item with a given
 // number (ascending from call to call).
 template <bool SEL>
 struct TreeWalk {
-    int C, b0, item0, part0;         // block of 32 requests: its first, and the items and parts before it
-    int items, parts;                // of the block
-    int r0, n, ctx, tiles, runs;     // this lane's request
+    int C, b0, item0, part0;             // block of 32 requests: its first, and the items and parts before it
+    int items, parts;                    // of the block
+    int id, r0, n, ctx, tiles, len, runs;  // this lane's request
     int excl_item, excl_part;
     __device__ void load(const TreeParams& p) {
-        const int b = b0 + (threadIdx.x & 31);
+        id = b0 + (threadIdx.x & 31);
         r0 = n = ctx = tiles = 0;
-        if (b < p.batch) {
-            const TreeSeq s = tree_seq(p, b);
+        if (id < p.batch) {
+            const TreeSeq s = tree_seq(p, id);
             r0 = s.r0;
             n = s.n;
             ctx = s.ctx;
             tiles = n > 0 ? tree_tiles<SEL>(p, s) : 0;
         }
     }
+    __device__ void sort() {  // longest first (a single block only), by a bitonic network
+        const int lane = threadIdx.x & 31;
+        unsigned key = (unsigned)tiles * 32u + (unsigned)(31 - lane);  // tiles < 2^26
+#pragma unroll 1
+        for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll 1
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                const unsigned other = __shfl_xor_sync(0xffffffffu, key, j);
+                const bool high = ((lane & j) == 0) == ((lane & k) == 0);  // keeps the larger
+                key = high ? max(key, other) : min(key, other);
+            }
+        const int from = 31 - (int)(key & 31);
+        id = __shfl_sync(0xffffffffu, id, from);
+        r0 = __shfl_sync(0xffffffffu, r0, from);
+        n = __shfl_sync(0xffffffffu, n, from);
+        ctx = __shfl_sync(0xffffffffu, ctx, from);
+        tiles = __shfl_sync(0xffffffffu, tiles, from);
+    }
     __device__ void count() {  // items and parts of the loaded block
-        runs = (tiles + C - 1) / C;
+        const int r = div_near(tiles + C - 1, C, 1.f / (float)C);
+        len = r > 1 ? (tiles + r - 1) / r : max(tiles, 1);
+        runs = (tiles + len - 1) / len;  // <= r: no run is empty
         const int it = n * runs, pt = runs > 1 ? it : 0;
         int si = it, sp = pt;
 #pragma unroll
@@ -303,10 +308,6 @@ struct TreeWalk {
         excl_part = sp - pt;
         items = __shfl_sync(0xffffffffu, si, 31);
         parts = __shfl_sync(0xffffffffu, sp, 31);
-    }
-    __device__ void start(const TreeParams& p) {
-        b0 = item0 = part0 = 0;
-        load(p);
     }
     __device__ bool next_block(const TreeParams& p) {
         item0 += items;
@@ -329,58 +330,55 @@ __device__ bool tree_item(const TreeParams& p, TreeWalk<SEL>& w, int item, TreeI
     const unsigned here = __ballot_sync(0xffffffffu, w.item0 + w.excl_item <= item && w.n * w.runs > 0);
     const int l = 31 - __clz((int)here);  // the last request that starts at or before the item
     const int local = item - (w.item0 + __shfl_sync(0xffffffffu, w.excl_item, l));
-    t.b = w.b0 + l;
+    t.b = __shfl_sync(0xffffffffu, w.id, l);
     t.r0 = __shfl_sync(0xffffffffu, w.r0, l);
     t.n = __shfl_sync(0xffffffffu, w.n, l);
     t.ctx = __shfl_sync(0xffffffffu, w.ctx, l);
     const int all = __shfl_sync(0xffffffffu, w.tiles, l), runs = __shfl_sync(0xffffffffu, w.runs, l);
+    const int len = __shfl_sync(0xffffffffu, w.len, l);
     const int run = local / t.n;  // the request's nodes side by side on one run of keys
     t.node = local - run * t.n;
-    t.tile0 = run * w.C;
-    t.tiles = min(w.C, all - t.tile0);
+    t.tile0 = run * len;
+    t.tiles = min(len, all - t.tile0);
     t.part = runs > 1 ? w.part0 + __shfl_sync(0xffffffffu, w.excl_part, l) + t.node * runs + run : -1;
     return true;
 }
 
 template <bool SEL>
-__global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
-    tree_attn_kernel(const TreeParams p, const __grid_constant__ TreeMaps tm) {
+__global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(const TreeParams p, const __grid_constant__ TreeMaps tm) {
     using L = TaLayout<SEL>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sK = smem_u32(smem), sP = smem_u32(smem + L::OFF_P);
     int4* items = reinterpret_cast<int4*>(smem + L::OFF_ITEM);  // (row or -1 = no more, tiles, part, unused)
     unsigned long long* see_sh = reinterpret_cast<unsigned long long*>(smem + L::OFF_SEE);
-    int* rows_sh = reinterpret_cast<int*>(smem + L::OFF_ROWS);
-    uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-    uint64_t* kfree = kfull + TA_NBUF;
-    uint64_t* sfull = kfree + TA_NBUF;
-    uint64_t* sfree = sfull + 2;
-    uint64_t* pready = sfree + 2;
+    uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);  // [entry][half]
+    uint64_t* kfree = kfull + 2 * TA_NBUF;
+    uint64_t* sfull = kfree + 2 * TA_NBUF;
+    uint64_t* pready = sfull + 2;
     uint64_t* pvdone = pready + 1;
     uint64_t* qtmem = pvdone + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
-    volatile int* go = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [2], by ring entry parity
-    int* chosen = reinterpret_cast<int*>(tmem_slot + 3);
+    int* longest_sh = reinterpret_cast<int*>(tmem_slot + 1);
+    volatile int* go = reinterpret_cast<volatile int*>(tmem_slot + 2);    // lists: [2], by the parity of the wait
     volatile int* info = reinterpret_cast<volatile int*>(tmem_slot + 4);  // lists: the item, for all gather threads
+    int* rows_sh = reinterpret_cast<int*>(smem + L::OFF_ROWS);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int b = 0; b < TA_NBUF; ++b) {
+        for (int b = 0; b < 2 * TA_NBUF; ++b) {
             mbar_init(kfull + b, SEL ? L::LOADERS : 1);
-            mbar_init(kfree + b, 1);  // the P.V commit; the MMA warp for a query entry
+            mbar_init(kfree + b, 1);  // the P.V commit of that half; the MMA warp for a query entry
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(sfull + b, 1);
-            mbar_init(sfree + b, 128);
-        }
+        mbar_init(sfull, 1);
+        mbar_init(sfull + 1, 1);
         mbar_init(pready, 128);
         mbar_init(pvdone, 1);
         mbar_init(qtmem, 128);
         fence_mbar_init();
     }
     if (warp == L::MMA_WARP) tmem_alloc(tmem_slot, 512);
-    if (warp == 4 && lane < (SEL ? 1 : 3))
+    if (warp == TA_LOAD_WARP && lane < (SEL ? 1 : 3))
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &tm.q : lane == 1 ? &tm.ckv : &tm.krot)) : "memory");
     tc_fence_before();
     __syncthreads();
@@ -388,104 +386,98 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
     pdl_trigger();
-    if (p.batch > 32) {
-        tree_schedule<SEL>(p, smem, chosen);
-        // the schedule's scratch becomes key tiles: order its generic accesses before TMA writes
-        fence_proxy_async_smem();
+    // The schedule: (nodes, tiles) of the requests, up to 32 by the producer warp, which keeps them sorted
+    // in registers; more by all threads, in the key tiles' space.
+    TreeCost* cost = reinterpret_cast<TreeCost*>(smem + L::OFF_P);
+    const bool many = p.batch > 32;
+    int2* tab = reinterpret_cast<int2*>(many ? smem : smem + L::OFF_P + sizeof(TreeCost));
+    TreeWalk<SEL> walk;
+    if (many) {
+        if (tid == 0) *longest_sh = 0;
+        __syncthreads();
+        int longest = 0;
+        for (int b = tid; b < p.batch; b += L::THREADS) {
+            const TreeSeq q = tree_seq(p, b);
+            const int t = q.n > 0 ? tree_tiles<SEL>(p, q) : 0;
+            tab[b] = make_int2(q.n, t);
+            longest = max(longest, t);
+        }
+        if (longest > 0) atomicMax(longest_sh, longest);
+    }
+    if (warp == TA_LOAD_WARP) {
+        walk.b0 = walk.item0 = walk.part0 = 0;
+        walk.load(p);
+        if (!many) {
+            if (p.batch > 1) walk.sort();
+            if (lane < p.batch) tab[lane] = make_int2(walk.n, walk.tiles);
+            if (lane == 0) *longest_sh = walk.tiles;
+        }
+    }
+    __syncthreads();
+    walk.C = tree_schedule(p, tab, *longest_sh, cost);
+    if (many) {
+        fence_proxy_async_smem();  // the table becomes key tiles: its generic accesses come before TMA writes
         __syncthreads();
     }
 
-    if (warp >= 4 && warp < L::MMA_WARP) {
-        // ---------------- producer ----------------
-        const int g = tid - 128;
-        TreeWalk<SEL> walk;
-        if (warp == 4) {
-            walk.start(p);
-            walk.C = p.batch > 32 ? *chosen : tree_schedule_warp(p, walk.n, walk.tiles);
-            walk.count();
-            if (blockIdx.x == gridDim.x - 1) {  // the parts of every node, for the merge
-                for (int r = lane; r < p.n_nodes; r += 32) p.node_tab[r] = make_int2(0, 0);
-                __syncwarp();
-                TreeWalk<SEL> w = walk;
-                do {
-                    if (w.runs > 1)
-                        for (int j = 0; j < w.n; ++j) p.node_tab[w.r0 + j] = make_int2(w.part0 + w.excl_part + j * w.runs, w.runs);
-                } while (w.next_block(p));
-            }
+    if (warp == TA_LOAD_WARP) {  // the producer, or the first gather warp
+        walk.count();
+        if (blockIdx.x == gridDim.x - 1) {  // the parts of every node, for the merge
+            for (int r = lane; r < p.n_nodes; r += 32) p.node_tab[r] = make_int2(0, 0);
+            __syncwarp();
+            TreeWalk<SEL> w = walk;
+            do {
+                if (w.runs > 1)
+                    for (int j = 0; j < w.n; ++j) p.node_tab[w.r0 + j] = make_int2(w.part0 + w.excl_part + j * w.runs, w.runs);
+            } while (w.next_block(p));
         }
-        int e = 0;  // ring entries issued
-        bool ok = true;
-        // Waits for ring entry e's space; all loader threads get the same answer.
-        auto acquire = [&]() -> bool {
-            const int b = e % TA_NBUF;
-            if constexpr (SEL) {
-                if (g == 0) go[e & 1] = e < TA_NBUF || mbar_wait_fast(kfree + b, (uint32_t)(e / TA_NBUF - 1) & 1u, 50) ? 1 : 0;
-                asm volatile("bar.sync 2, %0;" ::"n"(L::LOADERS) : "memory");
-                return go[e & 1] != 0;  // rewritten two entries on, behind the barrier in between
-            } else {
-                return e < TA_NBUF || mbar_wait_fast(kfree + b, (uint32_t)(e / TA_NBUF - 1) & 1u, 50);
-            }
-        };
-        int pend = -1;  // lists: the tile whose copies are in flight
-        auto flush = [&]() {
-            if constexpr (SEL) {
-                if (pend >= 0) {
-                    cp_async_wait<0>();
-                    fence_proxy_async_smem();
-                    mbar_arrive(kfull + pend);
-                    pend = -1;
+    }
+
+    if (warp >= TA_LOAD_WARP && warp < L::MMA_WARP) {
+        if constexpr (!SEL) {
+            // ---------------- producer (every key): one warp ----------------
+            int e = 0;  // ring entries issued
+            bool ok = true;
+            // A ring entry's half is free: its third-last use was consumed.
+            auto acquire = [&](int half) -> bool {
+                return e < TA_NBUF || mbar_wait_fast(kfree + 2 * (e % TA_NBUF) + half, (uint32_t)(e / TA_NBUF - 1) & 1u, 50);
+            };
+            auto arm = [&](int half, int bytes) {  // by lane 0; no bytes: arrives at once
+                uint64_t* bar = kfull + 2 * (e % TA_NBUF) + half;
+                if (lane == 0) {
+                    if (bytes > 0) mbar_expect_tx(bar, (uint32_t)bytes);
+                    else mbar_arrive(bar);
                 }
-            }
-        };
-        for (int item = blockIdx.x;; item += gridDim.x) {
-            TreeItem t;
-            bool more = true;
-            if (warp == 4) more = tree_item<SEL>(p, walk, item, t);
-            if constexpr (SEL) {
-                flush();
-                if (warp == 4 && lane == 0) {
-                    info[0] = more ? 1 : 0;
-                    if (more) {
-                        const int left = tree_list_n(p, t.r0 + t.node) - t.tile0 * TA_TILE;  // of the list, from this item on
-                        info[1] = t.b;
-                        info[2] = t.r0 + t.node;
-                        info[3] = t.ctx;
-                        info[4] = t.n;
-                        info[5] = t.tile0 * TA_TILE;
-                        info[6] = max(0, min(left, t.tiles * TA_TILE));
+                __syncwarp();
+            };
+            for (int k = 0; ok; ++k) {
+                TreeItem t{};
+                const bool more = tree_item<SEL>(p, walk, item_of(k), t);
+                const int row = t.r0 + t.node, n_tiles = t.tiles;
+                if (!(ok = acquire(0) && acquire(1))) break;
+                {
+                    const int b = e % TA_NBUF;
+                    if (lane == 0) items[b] = make_int4(more ? row : -1, n_tiles, t.part, 0);
+                    if (!more) {
+                        arm(0, 0);
+                        break;
                     }
+                    // the query, 64 heads x 576: nine boxes
+                    arm(0, 5 * L::CHUNK);
+                    arm(1, 4 * L::CHUNK);
+                    if (lane < AT_CHUNKS)
+                        tma_load2d(sK + b * L::TILE + lane * L::CHUNK, &tm.q, lane * 64, row * AT_H,
+                                   kfull + 2 * b + (lane >= 4 && lane < 8 ? 1 : 0));
+                    ++e;
                 }
-            }
-            if (!(ok = acquire())) break;  // also orders info[] for the gather threads
-            const int b = e % TA_NBUF;
-            if constexpr (SEL) more = info[0] != 0;
-            const int row = SEL ? info[2] : t.r0 + t.node;
-            const int n_keys = SEL ? info[6] : 0;
-            const int n_tiles = SEL ? (n_keys + TA_TILE - 1) / TA_TILE : t.tiles;
-            if (g == 0) items[b] = make_int4(more ? row : -1, n_tiles, t.part, 0);
-            if (!more) {
-                if (SEL || lane == 0) mbar_arrive(kfull + b);
-                ++e;
-                break;
-            }
-            // the query, 64 heads x 576: nine boxes
-            if (g == 0) {
-                mbar_expect_tx(kfull + b, L::TILE);
-                for (int c = 0; c < AT_CHUNKS; ++c)
-                    tma_load2d(sK + b * L::TILE + c * L::CHUNK, &tm.q, c * 64, row * AT_H, kfull + b);
-            } else if (SEL) {
-                mbar_arrive(kfull + b);
-            }
-            ++e;
-            if constexpr (!SEL) {
-                const int R = p.box_rows, nbox = TA_TILE / R;
                 const int* table = p.table + (long long)t.b * p.table_stride;
+                const int R = p.box_rows, nbox = TA_TILE / R;
                 // this lane's box of a tile: its page, loaded a tile ahead
                 int pos = t.tile0 * TA_TILE + lane * R, page = 0;
                 if (lane < nbox && pos < t.ctx + t.n) page = __ldg(table + pos / p.page_size);
                 const unsigned long long see = tree_mask_of(p, t.r0, t.n, t.node);
-                for (int i = 0; i < n_tiles; ++i, ++e) {
-                    const int pos0 = (t.tile0 + i) * TA_TILE, bb = e % TA_NBUF;
+                for (int i = 0; i < n_tiles && ok; ++i) {
+                    const int pos0 = (t.tile0 + i) * TA_TILE, b = e % TA_NBUF;
                     // its first slot, -1 past the request's rows or outside the pool
                     int slot = -1;
                     bool bad = false;
@@ -498,107 +490,202 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
                     if (lane < nbox && pos < t.ctx + t.n && i + 1 < n_tiles) page = __ldg(table + pos / p.page_size);
                     const int have = __popc(__ballot_sync(0xffffffffu, slot >= 0));
                     const unsigned lost = __ballot_sync(0xffffffffu, bad);
-                    if (!(ok = acquire())) break;
+                    const uint32_t tile = sK + b * L::TILE;
+                    if (!(ok = acquire(0))) break;
                     if (lane == 0) {
-                        const int k = pos0 - t.ctx;  // first key as a node number
-                        unsigned long long v = k >= 64 ? 0ull : k >= 0 ? see >> k : k <= -64 ? ~0ull : (see << -k) | ((1ull << -k) - 1);
+                        const int first = pos0 - t.ctx;  // first key as a node number
+                        unsigned long long v = first >= 64    ? 0ull
+                                               : first >= 0   ? see >> first
+                                               : first <= -64 ? ~0ull
+                                                              : (see << -first) | ((1ull << -first) - 1);
                         if (lost)
                             for (int j = 0; j < nbox; ++j)
                                 if ((lost >> j) & 1) v &= ~((R >= 64 ? ~0ull : (1ull << R) - 1) << (j * R));
-                        see_sh[bb] = v;
-                        if (have > 0) mbar_expect_tx(kfull + bb, (uint32_t)have * R * 128 * AT_CHUNKS);
-                        else mbar_arrive(kfull + bb);
+                        see_sh[b] = v;
                     }
-                    __syncwarp();
-                    const uint32_t tile = sK + bb * L::TILE;
-                    for (int x0 = 0; x0 < nbox * AT_CHUNKS; x0 += 32) {
-                        const int x = x0 + lane, j = x / AT_CHUNKS, c = x - j * AT_CHUNKS;
-                        const int y = __shfl_sync(0xffffffffu, slot, j & 31);
-                        if (x < nbox * AT_CHUNKS && y >= 0)
-                            tma_load2d(tile + c * L::CHUNK + j * R * 128, c < 8 ? &tm.ckv : &tm.krot, c < 8 ? c * 64 : 0, y, kfull + bb);
-                    }
+                    auto boxes = [&](int half) {  // columns 0-255 and the roped ones, or 256-511
+                        const int per = 5 - half;
+                        arm(half, have * R * 128 * per);
+                        for (int x0 = 0; x0 < nbox * per; x0 += 32) {
+                            const int x = x0 + lane, j = x / per, c = half ? 4 + x - j * per : x - j * per == 4 ? 8 : x - j * per;
+                            const int y = __shfl_sync(0xffffffffu, slot, j & 31);
+                            if (x < nbox * per && y >= 0)
+                                tma_load2d(tile + c * L::CHUNK + j * R * 128, c < 8 ? &tm.ckv : &tm.krot, c < 8 ? c * 64 : 0, y,
+                                           kfull + 2 * b + half);
+                        }
+                    };
+                    boxes(0);
+                    if (!(ok = acquire(1))) break;
+                    boxes(1);
+                    ++e;
                 }
-            } else {
-                const int qb = info[1], ctx = info[3], n = info[4];
-                if (warp == 4) {
-                    const unsigned long long see = tree_mask_of(p, t.r0, t.n, t.node);
+            }
+            if (!ok)  // copies in flight must land before the CTA leaves
+                for (int k = max(0, e - TA_NBUF); k <= e; ++k)
+                    for (int half = 0; half < 2; ++half) mbar_wait_fast(kfull + 2 * (k % TA_NBUF) + half, (uint32_t)(k / TA_NBUF) & 1u, 51);
+        } else {
+            // ---------------- gather (lists): all 8 warps ----------------
+            const int g = tid - 128;
+            int e = 0, waits = 0;  // ring entries issued, acquire calls
+            bool ok = true;
+            // A ring entry's half is free. One thread waits; all gather threads get the same answer.
+            auto acquire = [&](int half) -> bool {
+                const int x = waits++ & 1;
+                if (g == 0)
+                    go[x] = e < TA_NBUF || mbar_wait_fast(kfree + 2 * (e % TA_NBUF) + half, (uint32_t)(e / TA_NBUF - 1) & 1u, 50) ? 1 : 0;
+                asm volatile("bar.sync 2, %0;" ::"n"(L::LOADERS) : "memory");
+                return go[x] != 0;  // rewritten two calls on, behind the barrier in between
+            };
+            int pend = -1;  // ring slot whose copies are in flight, two groups (halves)
+            auto landed = [&](int half) {
+                fence_proxy_async_smem();
+                mbar_arrive(kfull + 2 * pend + half);
+            };
+            auto flush = [&]() {
+                if (pend < 0) return;
+                cp_async_wait<1>();
+                landed(0);
+                cp_async_wait<0>();
+                landed(1);
+                pend = -1;
+            };
+            const int r8 = g >> 3, seg = g & 7;  // this thread's 16 bytes of rows r8 and r8 + 32 of a tile
+            for (int k = 0; ok; ++k) {
+                TreeItem t{};
+                if (warp == TA_LOAD_WARP) {
+                    const bool more = tree_item<SEL>(p, walk, item_of(k), t);
+                    unsigned long long see = 0;
+                    int left = 0;  // entries of this item
+                    if (more) {
+                        left = max(0, min(tree_list_n(p, t.r0 + t.node) - t.tile0 * TA_TILE, t.tiles * TA_TILE));
+                        see = tree_mask_of(p, t.r0, t.n, t.node);
+                    }
                     if (lane == 0) {
-                        info[7] = (int)(unsigned)see;
-                        info[8] = (int)(unsigned)(see >> 32);
+                        info[0] = more ? t.r0 + t.node : -1;
+                        info[1] = t.b;
+                        info[2] = t.ctx;
+                        info[3] = t.n;
+                        info[4] = t.tile0 * TA_TILE;
+                        info[5] = left;
+                        info[6] = (int)(unsigned)see;
+                        info[7] = (int)(unsigned)(see >> 32);
                     }
                 }
-                const int* list = p.sel + (long long)row * p.sel_stride + info[5];
-                const int* table = p.table + (long long)qb * p.table_stride;
-                // the slot of this thread's key of tile i (threads 0-63), -1 when the row does not see it
-                asm volatile("bar.sync 2, %0;" ::"n"(L::LOADERS) : "memory");  // info[0..6] is read, info[7..8] written
-                const unsigned long long mine = (unsigned)info[7] | ((unsigned long long)(unsigned)info[8] << 32);
-                auto slot_of = [&](int i) -> int {
-                    const int k = i * TA_TILE + g;
-                    if (g >= TA_TILE || k >= n_keys) return -1;
-                    const int pos = __ldg(list + k);
-                    if (pos < 0 || pos >= ctx + n || (pos >= ctx && !((mine >> (pos - ctx)) & 1))) return -1;
-                    return page_slot(table, p.page_size, p.n_pages, pos, 46);
+                flush();
+                if (!(ok = acquire(0))) break;  // also orders info[]
+                const int row = info[0], left = info[5], n_tiles = (left + TA_TILE - 1) / TA_TILE, ctx = info[2], n = info[3];
+                const unsigned long long see = (unsigned)info[6] | ((unsigned long long)(unsigned)info[7] << 32);
+                const int* table = p.table + (long long)info[1] * p.table_stride;
+                const int* list = p.sel + (long long)max(row, 0) * p.sel_stride + info[4];
+                if (!(ok = acquire(1))) break;  // and info[] is read before the next item's
+                const int qb = e % TA_NBUF;
+                if (g == 0) items[qb] = make_int4(row, n_tiles, t.part, 0);
+                if (row < 0) {
+                    mbar_arrive(kfull + 2 * qb);
+                    break;
+                }
+                if (g == 0) {  // the query, 64 heads x 576: nine boxes
+                    mbar_expect_tx(kfull + 2 * qb, 5 * L::CHUNK);
+                    mbar_expect_tx(kfull + 2 * qb + 1, 4 * L::CHUNK);
+                    for (int c = 0; c < AT_CHUNKS; ++c)
+                        tma_load2d(sK + qb * L::TILE + c * L::CHUNK, &tm.q, c * 64, row * AT_H, kfull + 2 * qb + (c >= 4 && c < 8 ? 1 : 0));
+                } else {
+                    mbar_arrive(kfull + 2 * qb);
+                    mbar_arrive(kfull + 2 * qb + 1);
+                }
+                ++e;
+                // threads 0-63: the slot of a tile's key, -1 when the row does not see it; positions are loaded two
+                // tiles ahead, pages one
+                auto entry = [&](int j) -> int { return g < TA_TILE && j < left ? __ldg(list + j) : -1; };
+                auto page_of = [&](int& pos) -> int {
+                    const bool is = pos >= 0 && pos < ctx + n && (pos < ctx || ((see >> (pos - ctx)) & 1));
+                    if (!is) pos = -1;
+                    return is ? __ldg(table + pos / p.page_size) : 0;
                 };
-                int next = slot_of(0);
-                for (int i = 0; i < n_tiles; ++i, ++e) {
-                    const int bb = e % TA_NBUF;
+                int pos = entry(g), nxt = entry(g + TA_TILE), page = page_of(pos);
+                for (int i = 0; i < n_tiles; ++i) {
+                    const int b = e % TA_NBUF;
                     if (g < TA_TILE) {
-                        // rows_sh and see_sh of this entry were last read three entries ago, behind acquire's barrier
-                        const unsigned bits = __ballot_sync(0xffffffffu, next >= 0);
-                        rows_sh[bb * TA_TILE + g] = next;
-                        next = slot_of(i + 1);
-                        if (!(ok = acquire())) break;
-                        if (lane == 0) reinterpret_cast<volatile unsigned*>(see_sh + bb)[g >> 5] = bits;
-                    } else if (!(ok = acquire())) {
+                        int slot = -1;
+                        if (pos >= 0) {
+                            if (page < 0 || page >= p.n_pages) set_error(ERRC_BOUNDS, 46);
+                            else slot = page * p.page_size + pos % p.page_size;
+                        }
+                        // rows_sh and see_sh of this slot were last read three entries ago, behind acquire's barriers
+                        rows_sh[b * TA_TILE + g] = slot;
+                        const unsigned bits = __ballot_sync(0xffffffffu, slot >= 0);
+                        pos = nxt;
+                        page = page_of(pos);
+                        nxt = entry((i + 2) * TA_TILE + g);
+                        if (!(ok = acquire(0))) break;
+                        if (lane == 0) reinterpret_cast<volatile unsigned*>(see_sh + b)[g >> 5] = bits;
+                    } else if (!(ok = acquire(0))) {
                         break;
                     }
-                    const uint32_t tile = sK + bb * L::TILE;
-#pragma unroll 3
-                    for (int k2 = 0; k2 < AT_CHUNKS * TA_TILE * 8 / L::LOADERS; ++k2) {  // 18 pieces of 16 B a thread
-                        const int pid = k2 * L::LOADERS + g;
-                        const int c = pid / (TA_TILE * 8), rem = pid % (TA_TILE * 8);
-                        const int j = rem >> 3, seg = rem & 7;
-                        const int sl = rows_sh[bb * TA_TILE + j];
-                        const __nv_bfloat16* src = c < 8 ? p.c_kv + (long long)max(sl, 0) * p.ckv_row + c * 64 + seg * 8
-                                                         : p.k_rot + (long long)max(sl, 0) * p.krot_row + seg * 8;
-                        cp_async16(tile + c * L::CHUNK + sw128_off(j, seg), src, sl < 0 ? 0u : 16u);
+                    const uint32_t dst = sK + b * L::TILE + sw128_off(r8, seg);  // row r8 + 32 swizzles alike
+                    const int sl0 = rows_sh[b * TA_TILE + r8], sl1 = rows_sh[b * TA_TILE + r8 + 32];
+                    const uint32_t by0 = sl0 < 0 ? 0u : 16u, by1 = sl1 < 0 ? 0u : 16u;
+                    const __nv_bfloat16* src0 = p.c_kv + (long long)max(sl0, 0) * p.ckv_row + seg * 8;
+                    const __nv_bfloat16* src1 = p.c_kv + (long long)max(sl1, 0) * p.ckv_row + seg * 8;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        cp_async16(dst + c * L::CHUNK, src0 + c * 64, by0);
+                        cp_async16(dst + c * L::CHUNK + 32 * 128, src1 + c * 64, by1);
+                    }
+                    cp_async16(dst + 8 * L::CHUNK, p.k_rot + (long long)max(sl0, 0) * p.krot_row + seg * 8, by0);
+                    cp_async16(dst + 8 * L::CHUNK + 32 * 128, p.k_rot + (long long)max(sl1, 0) * p.krot_row + seg * 8, by1);
+                    cp_async_commit();
+                    if (pend >= 0) {
+                        cp_async_wait<2>();
+                        landed(0);
+                    }
+                    if (!(ok = acquire(1))) break;
+#pragma unroll
+                    for (int c = 4; c < 8; ++c) {
+                        cp_async16(dst + c * L::CHUNK, src0 + c * 64, by0);
+                        cp_async16(dst + c * L::CHUNK + 32 * 128, src1 + c * 64, by1);
                     }
                     cp_async_commit();
                     if (pend >= 0) {
-                        cp_async_wait<1>();
-                        fence_proxy_async_smem();
-                        mbar_arrive(kfull + pend);
+                        cp_async_wait<2>();
+                        landed(1);
                     }
-                    pend = bb;
+                    pend = b;
+                    ++e;
                 }
             }
-            if (!ok) break;
-        }
-        if (SEL) {
             cp_async_wait<0>();
-            if (ok) flush();
+            if (!ok && g == 0) {  // a query in flight must land before the CTA leaves
+                for (int k = 0; k < 2 * TA_NBUF; ++k) mbar_wait_fast(kfull + k, 0, 51);
+            }
         }
-        if (!ok && g == 0)  // copies in flight must land before the CTA leaves
-            for (int k = max(0, e - TA_NBUF); k < e; ++k) mbar_wait_fast(kfull + k % TA_NBUF, (uint32_t)(k / TA_NBUF) & 1u, 51);
     } else if (warp == L::MMA_WARP) {
         // ---------------- MMA ----------------
         const uint32_t tq = tmem + (16u << 16) + PF_TM_Q;
         int e = 0, gt = 0;  // ring entries and key tiles taken
+        // Tile g's scores go to S buffer g & 1: its reader of two tiles before is done (that tile's P.V was issued).
         auto issue_qk = [&](int entry, int g_) -> bool {
             const int b = entry % TA_NBUF, s = g_ & 1;
-            if (!mbar_wait_fast(kfull + b, (uint32_t)(entry / TA_NBUF) & 1u, 52)) return false;
-            if (g_ >= 2 && !mbar_wait_fast(sfree + s, (uint32_t)((g_ >> 1) - 1) & 1u, 53)) return false;
+            const uint32_t d = tmem + (16u << 16) + (uint32_t)(s * TA_TILE);
+            const uint64_t k0 = desc_sw128(sK + b * L::TILE, 16, 1024);
+            auto chunk = [&](int c) {
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)  // descriptors step in 16-byte units
+                    mma_bf16_ts(d, tq + (uint32_t)(c * 32 + kk * 8), k0 + ((c * L::CHUNK + kk * 32) >> 4), L::IDESC_QK,
+                                (c | kk) != 0 ? 1u : 0u);
+            };
+            if (!mbar_wait_fast(kfull + 2 * b, (uint32_t)(entry / TA_NBUF) & 1u, 52)) return false;
             tc_fence_after();
             if (elect_one()) {
-                const uint32_t d = tmem + (16u << 16) + (uint32_t)(s * TA_TILE);
-                const uint64_t k0 = desc_sw128(sK + b * L::TILE, 16, 1024);
 #pragma unroll
-                for (int c = 0; c < AT_CHUNKS; ++c) {
+                for (int c = 0; c < 4; ++c) chunk(c);
+                chunk(8);
+            }
+            if (!mbar_wait_fast(kfull + 2 * b + 1, (uint32_t)(entry / TA_NBUF) & 1u, 53)) return false;
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)  // descriptors step in 16-byte units
-                        mma_bf16_ts(d, tq + (uint32_t)(c * 32 + kk * 8), k0 + ((c * L::CHUNK + kk * 32) >> 4), L::IDESC_QK,
-                                    (c | kk) != 0 ? 1u : 0u);
-                }
+                for (int c = 4; c < 8; ++c) chunk(c);
                 mma_commit(sfull + s);
             }
             __syncwarp();
@@ -611,13 +698,13 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
             if (elect_one()) {
                 const uint64_t p0 = desc_sw128(sP, 16, 1024), v0 = desc_sw128(sK + b * L::TILE, L::CHUNK, 1024);
 #pragma unroll
-                for (int ks = 0; ks < TA_TILE / 16; ++ks) {
+                for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
+                    for (int ks = 0; ks < TA_TILE / 16; ++ks)
                         mma_bf16(tmem + (uint32_t)(half * 256), p0 + ks * 2, v0 + ((4 * half * L::CHUNK + ks * 2048) >> 4),
                                  L::IDESC_PV, (!first || ks > 0) ? 1u : 0u);
+                    mma_commit(kfree + 2 * b + half);
                 }
-                mma_commit(kfree + b);
                 mma_commit(pvdone);
             }
             __syncwarp();
@@ -626,11 +713,14 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
         bool ok = true;
         for (int it = 0; ok; ++it) {
             const int qb = e % TA_NBUF;
-            if (!(ok = mbar_wait_fast(kfull + qb, (uint32_t)(e / TA_NBUF) & 1u, 55))) break;
+            if (!(ok = mbar_wait_fast(kfull + 2 * qb, (uint32_t)(e / TA_NBUF) & 1u, 55))) break;
             const int4 t = items[qb];
             if (t.x < 0) break;
             if (!(ok = mbar_wait_fast(qtmem, (uint32_t)it & 1u, 56))) break;  // the query is in tensor memory
-            if (elect_one()) mbar_arrive(kfree + qb);
+            if (elect_one()) {
+                mbar_arrive(kfree + 2 * qb);
+                mbar_arrive(kfree + 2 * qb + 1);
+            }
             ++e;
             const int n = t.y;
             if (n > 0) ok = issue_qk(e, gt);
@@ -652,9 +742,10 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
         bool ok = true;
         while (ok) {
             const int qb = e % TA_NBUF;
-            if (!(ok = mbar_wait_fast(kfull + qb, (uint32_t)(e / TA_NBUF) & 1u, 57))) break;
+            if (!(ok = mbar_wait_fast(kfull + 2 * qb, (uint32_t)(e / TA_NBUF) & 1u, 57))) break;
             const int4 t = items[qb];
             if (t.x >= 0) {
+                if (!(ok = mbar_wait_fast(kfull + 2 * qb + 1, (uint32_t)(e / TA_NBUF) & 1u, 57))) break;
                 // The next query into tensor memory: every QK of the item before is done (its scores were read).
                 const uint32_t src0 = sK + qb * L::TILE + (uint32_t)h * 128u;
 #pragma unroll 3
@@ -689,56 +780,48 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
                     if (out_part >= 0) p.lse_part[(long long)out_part * AT_H + h] = lse;
                     else if (p.lse) p.lse[(long long)out_row * AT_H + h] = lse;
                 }
-                // A warp's 16 heads pass through its own 2 KB of P's space (P.V is done with it), 128 bytes
-                // a head at a time, so that each store instruction writes four whole 128-byte lines: an item's
-                // output takes about 2,500 cycles instead of 11,000 with every thread storing its own columns.
-                const long long at = (out_part >= 0 ? (long long)out_part : (long long)out_row) * AT_H + 16 * warp;
-                const uint32_t mine = sP + (uint32_t)h * 128u, base = sP + (uint32_t)(16 * warp) * 128u;
+                // O leaves straight from registers in the fragment shape: four threads write whole 32-byte
+                // sectors of a head's row, and nothing waits (staging through shared memory or every thread
+                // storing its own run of columns took 7,000 and 11,000 cycles an item).
+                const long long at = (out_part >= 0 ? (long long)out_part : (long long)out_row) * AT_H + 16 * warp + (lane >> 2);
+                const float inv0 = __shfl_sync(0xffffffffu, inv, lane >> 2), inv1 = __shfl_sync(0xffffffffu, inv, (lane >> 2) + 8);
+                // an empty row (l = 0) has inv 0, but its O may hold anything
+                const bool any0 = __shfl_sync(0xffffffffu, (int)any, lane >> 2), any1 = __shfl_sync(0xffffffffu, (int)any, (lane >> 2) + 8);
                 const bool narrow = out_part < 0 && p.ctx_bf16;
-                char* out = narrow ? reinterpret_cast<char*>(static_cast<__nv_bfloat16*>(p.ctx) + at * AT_DV)
-                                   : reinterpret_cast<char*>((out_part >= 0 ? p.o_part : static_cast<float*>(p.ctx)) + at * AT_DV);
-                const int row_bytes = narrow ? AT_DV * 2 : AT_DV * 4;
-                auto store = [&](int byte0) {  // the staged 16 x 128 bytes to columns from byte0 on
-                    __syncwarp();
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int r = 4 * k + (lane >> 3), seg = lane & 7;
-                        const uint4 x = lds_v4(base + (uint32_t)r * 128u + (uint32_t)((seg ^ r) & 7) * 16u);
-                        *reinterpret_cast<uint4*>(out + (long long)r * row_bytes + byte0 + seg * 16) = x;
-                    }
-                    __syncwarp();
-                };
-                if (narrow) {
+                float* of = (out_part >= 0 ? p.o_part : static_cast<float*>(p.ctx)) + at * AT_DV + 2 * (lane & 3);
+                const bool odd = lane & 1;
+                __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(p.ctx) + at * AT_DV + (odd ? 8 : 0) + 4 * ((lane & 3) >> 1);
 #pragma unroll 1
-                    for (int c = 0; c < AT_DV; c += 64) {
-                        float ov[32];
-                        tmem_ld16x2_32<32>(tmem + lane_o + (uint32_t)c, ov);
+                for (int c = 0; c < AT_DV; c += 64) {
+                    float ov[32];
+                    tmem_ld16x256_8(tmem + lane_o + (uint32_t)c, ov);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            uint32_t w[4];
+                    for (int x = 0; x < 32; x += 4) {
+                        ov[x] = any0 ? ov[x] * inv0 : 0.f;
+                        ov[x + 1] = any0 ? ov[x + 1] * inv0 : 0.f;
+                        ov[x + 2] = any1 ? ov[x + 2] * inv1 : 0.f;
+                        ov[x + 3] = any1 ? ov[x + 3] * inv1 : 0.f;
+                    }
+                    if (narrow) {
+                        // two groups of 8 columns at a time: neighbours trade, so that an even thread has four
+                        // consecutive columns of the first group and an odd one of the second
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                const float a = ov[8 * k + 2 * x], b = ov[8 * k + 2 * x + 1];
-                                const __nv_bfloat162 b2 = __floats2bfloat162_rn(any ? a * inv : 0.f, any ? b * inv : 0.f);
-                                w[x] = *reinterpret_cast<const uint32_t*>(&b2);
+                        for (int x = 0; x < 32; x += 8) {
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const __nv_bfloat162 f0 = __floats2bfloat162_rn(ov[x + 2 * half], ov[x + 2 * half + 1]);
+                                const __nv_bfloat162 f1 = __floats2bfloat162_rn(ov[x + 4 + 2 * half], ov[x + 5 + 2 * half]);
+                                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(&f0), w1 = *reinterpret_cast<const uint32_t*>(&f1);
+                                const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? w0 : w1, 1);
+                                *reinterpret_cast<uint2*>(ob + half * 8 * AT_DV + c + 2 * x) = odd ? make_uint2(got, w1) : make_uint2(w0, got);
                             }
-                            sts_v4(mine + (uint32_t)(((hi_half ? 4 : 0) + k) ^ (h & 7)) * 16u, make_uint4(w[0], w[1], w[2], w[3]));
                         }
-                        store(c * 2);
-                    }
-                } else {
-#pragma unroll 1
-                    for (int c = 0; c < AT_DV; c += 32) {
-                        float ov[16];
-                        tmem_ld16x2_16<16>(tmem + lane_o + (uint32_t)c, ov);
+                    } else {
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) ov[k] = any ? ov[k] * inv : 0.f;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            sts_v4(mine + (uint32_t)(((hi_half ? 4 : 0) + k) ^ (h & 7)) * 16u,
-                                   make_uint4(__float_as_uint(ov[4 * k]), __float_as_uint(ov[4 * k + 1]),
-                                              __float_as_uint(ov[4 * k + 2]), __float_as_uint(ov[4 * k + 3])));
-                        store(c * 4);
+                        for (int x = 0; x < 32; x += 4) {
+                            *reinterpret_cast<float2*>(of + c + 2 * x) = make_float2(ov[x], ov[x + 1]);
+                            *reinterpret_cast<float2*>(of + 8 * AT_DV + c + 2 * x) = make_float2(ov[x + 2], ov[x + 3]);
+                        }
                     }
                 }
                 tc_fence_before();  // these reads come before the next P.V (ordered by pready)
@@ -750,14 +833,12 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
             l_run = 0.f;
             for (int i = 0; i < t.y && ok; ++i, ++e, ++gt) {
                 const int s = gt & 1, b = e % TA_NBUF;
-                if (!(ok = mbar_wait_fast(kfull + b, (uint32_t)(e / TA_NBUF) & 1u, 59))) break;  // orders see_sh
+                if (!(ok = mbar_wait_fast(kfull + 2 * b, (uint32_t)(e / TA_NBUF) & 1u, 59))) break;  // orders see_sh
                 const unsigned long long see = see_sh[b];
                 if (!(ok = mbar_wait_fast(sfull + s, (uint32_t)(gt >> 1) & 1u, 60))) break;
                 tc_fence_after();
                 float sv[32];
                 tmem_ld16x2_32<32>(tmem + lane_s + (uint32_t)(s * TA_TILE), sv);
-                tc_fence_before();
-                mbar_arrive(sfree + s);
                 float tmax = -INFINITY;
                 if (see == ~0ull) {
 #pragma unroll
@@ -772,15 +853,13 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1)
                         sv[j] = (bits >> j) & 1u ? sv[j] * p.scale_log2 : -INFINITY;
                         tmax = fmaxf(tmax, sv[j]);
                     }
-                    if constexpr (!SEL) {
-                        // An unseen row may hold anything (0 x NaN is NaN): its values become zeros
-                        // before P.V reads them. Lists load zeros for such rows.
-                        for (int j = warp; j < TA_TILE; j += 4) {
-                            if ((see >> j) & 1) continue;
-                            const uint32_t dst = sK + b * L::TILE + (uint32_t)(lane >> 3) * L::CHUNK + (uint32_t)j * 128u + (uint32_t)(lane & 7) * 16u;
-                            sts_v4(dst, make_uint4(0, 0, 0, 0));
-                            sts_v4(dst + 4 * L::CHUNK, make_uint4(0, 0, 0, 0));
-                        }
+                    // An unseen row may hold anything (0 x NaN is NaN): its values become zeros
+                    // before P.V reads them.
+                    for (int j = warp; j < TA_TILE; j += 4) {
+                        if ((see >> j) & 1) continue;
+                        const uint32_t dst = sK + b * L::TILE + (uint32_t)(lane >> 3) * L::CHUNK + (uint32_t)j * 128u + (uint32_t)(lane & 7) * 16u;
+                        sts_v4(dst, make_uint4(0, 0, 0, 0));
+                        sts_v4(dst + 4 * L::CHUNK, make_uint4(0, 0, 0, 0));
                     }
                 }
                 tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 16));
