@@ -465,9 +465,12 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     // the query, 64 heads x 576: nine boxes
                     arm(0, 5 * L::CHUNK);
                     arm(1, 4 * L::CHUNK);
-                    if (lane < AT_CHUNKS)
-                        tma_load2d(sK + b * L::TILE + lane * L::CHUNK, &tm.q, lane * 64, row * AT_H,
-                                   kfull + 2 * b + (lane >= 4 && lane < 8 ? 1 : 0));
+                    if (elect_one()) {
+#pragma unroll
+                        for (int c = 0; c < AT_CHUNKS; ++c)
+                            tma_load2d(sK + b * L::TILE + c * L::CHUNK, &tm.q, c * 64, row * AT_H, kfull + 2 * b + (c >= 4 && c < 8 ? 1 : 0));
+                    }
+                    __syncwarp();
                     ++e;
                 }
                 const int* table = p.table + (long long)t.b * p.table_stride;
@@ -503,16 +506,23 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                                 if ((lost >> j) & 1) v &= ~((R >= 64 ? ~0ull : (1ull << R) - 1) << (j * R));
                         see_sh[b] = v;
                     }
-                    auto boxes = [&](int half) {  // columns 0-255 and the roped ones, or 256-511
-                        const int per = 5 - half;
-                        arm(half, have * R * 128 * per);
-                        for (int x0 = 0; x0 < nbox * per; x0 += 32) {
-                            const int x = x0 + lane, j = x / per, c = half ? 4 + x - j * per : x - j * per == 4 ? 8 : x - j * per;
-                            const int y = __shfl_sync(0xffffffffu, slot, j & 31);
-                            if (x < nbox * per && y >= 0)
-                                tma_load2d(tile + c * L::CHUNK + j * R * 128, c < 8 ? &tm.ckv : &tm.krot, c < 8 ? c * 64 : 0, y,
-                                           kfull + 2 * b + half);
+                    // columns 0-255 and the roped ones, or 256-511, by one elected thread (the coordinates of
+                    // a TMA instruction are uniform registers: lanes issuing their own cost 75 cycles a box)
+                    auto boxes = [&](int half) {
+                        arm(half, have * R * 128 * (5 - half));
+                        uint64_t* bar = kfull + 2 * b + half;
+#pragma unroll 1
+                        for (int j = 0; j < nbox; ++j) {
+                            const int y = __shfl_sync(0xffffffffu, slot, j);
+                            const uint32_t dst = tile + (uint32_t)(j * R * 128);
+                            if (y >= 0 && elect_one()) {
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    tma_load2d(dst + (4 * half + c) * L::CHUNK, &tm.ckv, (4 * half + c) * 64, y, bar);
+                                if (half == 0) tma_load2d(dst + 8 * L::CHUNK, &tm.krot, 0, y, bar);
+                            }
                         }
+                        __syncwarp();
                     };
                     boxes(0);
                     if (!(ok = acquire(1))) break;
