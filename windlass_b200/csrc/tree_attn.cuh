@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
     volatile int* go = reinterpret_cast<volatile int*>(tmem_slot + 2);    // lists: [2], by the parity of the wait
     volatile int* info = reinterpret_cast<volatile int*>(tmem_slot + 4);  // lists: the item, for all gather threads
     int* rows_sh = reinterpret_cast<int*>(smem + L::OFF_ROWS);
+    volatile int* slots_sh = info;  // dense: first slots of a tile's boxes
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -442,14 +443,6 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
             auto acquire = [&](int half) -> bool {
                 return e < TA_NBUF || mbar_wait_fast(kfree + 2 * (e % TA_NBUF) + half, (uint32_t)(e / TA_NBUF - 1) & 1u, 50);
             };
-            auto arm = [&](int half, int bytes) {  // by lane 0; no bytes: arrives at once
-                uint64_t* bar = kfull + 2 * (e % TA_NBUF) + half;
-                if (lane == 0) {
-                    if (bytes > 0) mbar_expect_tx(bar, (uint32_t)bytes);
-                    else mbar_arrive(bar);
-                }
-                __syncwarp();
-            };
             for (int k = 0; ok; ++k) {
                 TreeItem t{};
                 const bool more = tree_item<SEL>(p, walk, item_of(k), t);
@@ -458,64 +451,74 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                 {
                     const int b = e % TA_NBUF;
                     if (lane == 0) items[b] = make_int4(more ? row : -1, n_tiles, t.part, 0);
-                    if (!more) {
-                        arm(0, 0);
-                        break;
-                    }
-                    // the query, 64 heads x 576: nine boxes
-                    arm(0, 5 * L::CHUNK);
-                    arm(1, 4 * L::CHUNK);
+                    __syncwarp();
                     if (elect_one()) {
+                        if (more) {  // the query, 64 heads x 576: nine boxes
+                            mbar_expect_tx(kfull + 2 * b, 5 * L::CHUNK);
+                            mbar_expect_tx(kfull + 2 * b + 1, 4 * L::CHUNK);
 #pragma unroll
-                        for (int c = 0; c < AT_CHUNKS; ++c)
-                            tma_load2d(sK + b * L::TILE + c * L::CHUNK, &tm.q, c * 64, row * AT_H, kfull + 2 * b + (c >= 4 && c < 8 ? 1 : 0));
+                            for (int c = 0; c < AT_CHUNKS; ++c)
+                                tma_load2d(sK + b * L::TILE + c * L::CHUNK, &tm.q, c * 64, row * AT_H,
+                                           kfull + 2 * b + (c >= 4 && c < 8 ? 1 : 0));
+                        } else {
+                            mbar_arrive(kfull + 2 * b);
+                        }
                     }
                     __syncwarp();
+                    if (!more) break;
                     ++e;
                 }
                 const int* table = p.table + (long long)t.b * p.table_stride;
                 const int R = p.box_rows, nbox = TA_TILE / R;
-                // this lane's box of a tile: its page, loaded a tile ahead
-                int pos = t.tile0 * TA_TILE + lane * R, page = 0;
-                if (lane < nbox && pos < t.ctx + t.n) page = __ldg(table + pos / p.page_size);
+                // this lane's box of a tile: its page (loaded a tile ahead) and its first row there; a tile on is
+                // `hop` pages and `rest` rows on
+                const int hop = TA_TILE / p.page_size, rest = TA_TILE % p.page_size, end = t.ctx + t.n;
+                int pos = t.tile0 * TA_TILE + lane * R, at = pos / p.page_size, off = pos - at * p.page_size;
+                bool mine = lane < nbox && pos < end;
+                int page = mine ? __ldg(table + at) : 0;
                 const unsigned long long see = tree_mask_of(p, t.r0, t.n, t.node);
                 for (int i = 0; i < n_tiles && ok; ++i) {
                     const int pos0 = (t.tile0 + i) * TA_TILE, b = e % TA_NBUF;
                     // its first slot, -1 past the request's rows or outside the pool
-                    int slot = -1;
-                    bool bad = false;
-                    if (lane < nbox && pos < t.ctx + t.n) {
-                        bad = page < 0 || page >= p.n_pages;
-                        if (bad) set_error(ERRC_BOUNDS, 46);
-                        else slot = page * p.page_size + pos % p.page_size;
-                    }
+                    const bool bad = mine && (page < 0 || page >= p.n_pages);
+                    if (bad) set_error(ERRC_BOUNDS, 46);
+                    const int slot = mine && !bad ? page * p.page_size + off : -1;
                     pos += TA_TILE;
-                    if (lane < nbox && pos < t.ctx + t.n && i + 1 < n_tiles) page = __ldg(table + pos / p.page_size);
+                    at += hop;
+                    off += rest;
+                    if (off >= p.page_size) {
+                        off -= p.page_size;
+                        ++at;
+                    }
+                    mine = lane < nbox && pos < end;
+                    if (mine && i + 1 < n_tiles) page = __ldg(table + at);
                     const int have = __popc(__ballot_sync(0xffffffffu, slot >= 0));
                     const unsigned lost = __ballot_sync(0xffffffffu, bad);
-                    const uint32_t tile = sK + b * L::TILE;
-                    if (!(ok = acquire(0))) break;
-                    if (lane == 0) {
+                    unsigned long long v = ~0ull;
+                    if (pos0 + TA_TILE > t.ctx) {  // drafted rows, or none
                         const int first = pos0 - t.ctx;  // first key as a node number
-                        unsigned long long v = first >= 64    ? 0ull
-                                               : first >= 0   ? see >> first
-                                               : first <= -64 ? ~0ull
-                                                              : (see << -first) | ((1ull << -first) - 1);
-                        if (lost)
-                            for (int j = 0; j < nbox; ++j)
-                                if ((lost >> j) & 1) v &= ~((R >= 64 ? ~0ull : (1ull << R) - 1) << (j * R));
-                        see_sh[b] = v;
+                        v = first >= 64 ? 0ull : first >= 0 ? see >> first : (see << -first) | ((1ull << -first) - 1);
                     }
-                    // columns 0-255 and the roped ones, or 256-511, by one elected thread (the coordinates of
-                    // a TMA instruction are uniform registers: lanes issuing their own cost 75 cycles a box)
+                    if (lost)
+                        for (int j = 0; j < nbox; ++j)
+                            if ((lost >> j) & 1) v &= ~((R >= 64 ? ~0ull : (1ull << R) - 1) << (j * R));
+                    if (lane < 8) slots_sh[lane] = slot;
+                    if (!(ok = acquire(0))) break;
+                    if (lane == 0) see_sh[b] = v;
+                    __syncwarp();
+                    // Columns 0-255 and the roped ones, then 256-511, all boxes by one elected thread: a TMA
+                    // instruction takes its coordinates from uniform registers, and lanes issuing a box each, or a
+                    // shuffle per box, took 75 and 60 cycles a box instead of 25.
                     auto boxes = [&](int half) {
-                        arm(half, have * R * 128 * (5 - half));
                         uint64_t* bar = kfull + 2 * b + half;
+                        if (elect_one()) {
+                            if (have > 0) mbar_expect_tx(bar, (uint32_t)(have * R * 128 * (5 - half)));
+                            else mbar_arrive(bar);
+                            uint32_t dst = sK + b * L::TILE;
 #pragma unroll 1
-                        for (int j = 0; j < nbox; ++j) {
-                            const int y = __shfl_sync(0xffffffffu, slot, j);
-                            const uint32_t dst = tile + (uint32_t)(j * R * 128);
-                            if (y >= 0 && elect_one()) {
+                            for (int j = 0; j < nbox; ++j, dst += R * 128) {
+                                const int y = slots_sh[j];
+                                if (y < 0) continue;
 #pragma unroll
                                 for (int c = 0; c < 4; ++c)
                                     tma_load2d(dst + (4 * half + c) * L::CHUNK, &tm.ckv, (4 * half + c) * 64, y, bar);
