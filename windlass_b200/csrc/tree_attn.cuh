@@ -344,6 +344,28 @@ __device__ bool tree_item(const TreeParams& p, TreeWalk<SEL>& w, int item, TreeI
     return true;
 }
 
+// One half of a key tile (columns 0-255 and the roped ones, or 256-511) in NB
+// boxes, by one thread: column by column, the boxes' rows in registers. A TMA
+// instruction takes its coordinates from uniform registers; with lanes issuing a
+// box each, or a branch and a shared-memory read per box, an instruction takes
+// 75 and 42 cycles, like this 17 to 30.
+template <int NB>
+__device__ __forceinline__ void tree_boxes(const TreeMaps& tm, uint32_t dst, int half, const volatile int* rows, uint64_t* bar) {
+    constexpr uint32_t CHUNK = TA_TILE * 128, BOX = CHUNK / NB;
+    int y[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) y[j] = rows[j];
+#pragma unroll(NB <= 2 ? 4 : 1)
+    for (int c = 4 * half; c < 4 * half + 4; ++c) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) tma_load2d(dst + c * CHUNK + j * BOX, &tm.ckv, c * 64, y[j], bar);
+    }
+    if (half == 0) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) tma_load2d(dst + 8 * CHUNK + j * BOX, &tm.krot, 0, y[j], bar);
+    }
+}
+
 template <bool SEL>
 __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(const TreeParams p, const __grid_constant__ TreeMaps tm) {
     using L = TaLayout<SEL>;
@@ -479,10 +501,10 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                 const unsigned long long see = tree_mask_of(p, t.r0, t.n, t.node);
                 for (int i = 0; i < n_tiles && ok; ++i) {
                     const int pos0 = (t.tile0 + i) * TA_TILE, b = e % TA_NBUF;
-                    // its first slot, -1 past the request's rows or outside the pool
+                    // its first slot; behind the pool (read as zeros) past the request's rows or for a bad page
                     const bool bad = mine && (page < 0 || page >= p.n_pages);
                     if (bad) set_error(ERRC_BOUNDS, 46);
-                    const int slot = mine && !bad ? page * p.page_size + off : -1;
+                    const int slot = mine && !bad ? page * p.page_size + off : p.n_pages * p.page_size;
                     pos += TA_TILE;
                     at += hop;
                     off += rest;
@@ -492,7 +514,6 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     }
                     mine = lane < nbox && pos < end;
                     if (mine && i + 1 < n_tiles) page = __ldg(table + at);
-                    const int have = __popc(__ballot_sync(0xffffffffu, slot >= 0));
                     const unsigned lost = __ballot_sync(0xffffffffu, bad);
                     unsigned long long v = ~0ull;
                     if (pos0 + TA_TILE > t.ctx) {  // drafted rows, or none
@@ -506,24 +527,16 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     if (!(ok = acquire(0))) break;
                     if (lane == 0) see_sh[b] = v;
                     __syncwarp();
-                    // Columns 0-255 and the roped ones, then 256-511, all boxes by one elected thread: a TMA
-                    // instruction takes its coordinates from uniform registers, and lanes issuing a box each, or a
-                    // shuffle per box, took 75 and 60 cycles a box instead of 25.
+                    // columns 0-255 and the roped ones, then 256-511
                     auto boxes = [&](int half) {
-                        uint64_t* bar = kfull + 2 * b + half;
                         if (elect_one()) {
-                            if (have > 0) mbar_expect_tx(bar, (uint32_t)(have * R * 128 * (5 - half)));
-                            else mbar_arrive(bar);
-                            uint32_t dst = sK + b * L::TILE;
-#pragma unroll 1
-                            for (int j = 0; j < nbox; ++j, dst += R * 128) {
-                                const int y = slots_sh[j];
-                                if (y < 0) continue;
-#pragma unroll
-                                for (int c = 0; c < 4; ++c)
-                                    tma_load2d(dst + (4 * half + c) * L::CHUNK, &tm.ckv, (4 * half + c) * 64, y, bar);
-                                if (half == 0) tma_load2d(dst + 8 * L::CHUNK, &tm.krot, 0, y, bar);
-                            }
+                            uint64_t* bar = kfull + 2 * b + half;
+                            mbar_expect_tx(bar, (uint32_t)((5 - half) * L::CHUNK));
+                            const uint32_t dst = sK + b * L::TILE;
+                            if (nbox == 1) tree_boxes<1>(tm, dst, half, slots_sh, bar);
+                            else if (nbox == 2) tree_boxes<2>(tm, dst, half, slots_sh, bar);
+                            else if (nbox == 4) tree_boxes<4>(tm, dst, half, slots_sh, bar);
+                            else tree_boxes<8>(tm, dst, half, slots_sh, bar);
                         }
                         __syncwarp();
                     };
