@@ -72,6 +72,8 @@ struct TreeMaps {
     CUtensorMap q;     // {576, 64 n_nodes}, box {64, 64}
     CUtensorMap ckv;   // {512, slots}, box {64, box_rows}
     CUtensorMap krot;  // {64, slots}, box {64, box_rows}
+    CUtensorMap part;  // the partials {512, 64 parts} fp32, box {32, 16}
+    CUtensorMap out;   // ctx {512, 64 n_nodes}, box of 128 bytes x 16 rows
 };
 
 // A request's rows and context; n = 0 (and the error word) when they are out of range.
@@ -188,12 +190,12 @@ __device__ __forceinline__ int tree_candidate(int c) { return c < 32 ? c + 1 : 3
 __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* tab, int longest, TreeCost* acc) {
     const int cand = threadIdx.x % TA_CANDS, grp = threadIdx.x / TA_CANDS, G = gridDim.x;
     const int per = (p.batch + 2) / 3, b0 = min(grp * per, p.batch), b1 = min(b0 + per, p.batch);
-    const int s = tree_candidate(cand), C = max(1, (longest + s - 1) / s);
-    const float inv = 1.f / (float)C;
+    const int s = tree_candidate(cand), C = max(1, div_near(longest + s - 1, s, __fdividef(1.f, (float)s)));
+    const float inv = __fdividef(1.f, (float)C);
     const bool mine = threadIdx.x < TA_SCHED_THREADS;
     if (mine) {
         int items = 0, parts = 0;
-#pragma unroll 1
+#pragma unroll 2
         for (int b = b0; b < b1; ++b) {
             const int2 v = tab[b];
             const int r = div_near(v.y + C - 1, C, inv);
@@ -208,7 +210,7 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
         const int all = acc->items[0][cand] + acc->items[1][cand] + acc->items[2][cand], full = all / G * G;
         int seen = (grp > 0 ? acc->items[0][cand] : 0) + (grp > 1 ? acc->items[1][cand] : 0);
         float sum = 0.f, last = 0.f;
-#pragma unroll 1
+#pragma unroll 2
         for (int b = b0; b < b1; ++b) {
             const int2 v = tab[b];
             const int r = div_near(v.y + C - 1, C, inv), it = v.x * r;
@@ -226,10 +228,11 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
     const int lane = threadIdx.x & 31;
     float best = 3e38f;
     int best_s = 1;
-#pragma unroll 1
+    const float inv_g = __fdividef(1.f, (float)G);
+#pragma unroll
     for (int c = lane; c < TA_CANDS; c += 32) {
         const int n_parts = acc->parts[0][c] + acc->parts[1][c] + acc->parts[2][c];
-        const float cost = (acc->sum[0][c] + acc->sum[1][c] + acc->sum[2][c]) / (float)G +
+        const float cost = (acc->sum[0][c] + acc->sum[1][c] + acc->sum[2][c]) * inv_g +
                            fmaxf(fmaxf(acc->last[0][c], acc->last[1][c]), acc->last[2][c]) + (float)n_parts * TA_PART_COST;
         if (n_parts <= p.parts_max && cost < best) {
             best = cost;
@@ -245,7 +248,7 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
             best_s = t;
         }
     }
-    return max(1, (longest + best_s - 1) / best_s);
+    return max(1, div_near(longest + best_s - 1, best_s, __fdividef(1.f, (float)best_s)));
 }
 // A CTA's item of round k: the CTAs take them forth and back.
 __device__ __forceinline__ int item_of(int k) {
@@ -291,9 +294,9 @@ struct TreeWalk {
         tiles = __shfl_sync(0xffffffffu, tiles, from);
     }
     __device__ void count() {  // items and parts of the loaded block
-        const int r = div_near(tiles + C - 1, C, 1.f / (float)C);
-        len = r > 1 ? (tiles + r - 1) / r : max(tiles, 1);
-        runs = (tiles + len - 1) / len;  // <= r: no run is empty
+        const int r = div_near(tiles + C - 1, C, __fdividef(1.f, (float)C));
+        len = r > 1 ? div_near(tiles + r - 1, r, __fdividef(1.f, (float)r)) : max(tiles, 1);
+        runs = div_near(tiles + len - 1, len, __fdividef(1.f, (float)len));  // <= r: no run is empty
         const int it = n * runs, pt = runs > 1 ? it : 0;
         int si = it, sp = pt;
 #pragma unroll
@@ -384,6 +387,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
     int* longest_sh = reinterpret_cast<int*>(tmem_slot + 1);
     volatile int* go = reinterpret_cast<volatile int*>(tmem_slot + 2);    // lists: [2], by the parity of the wait
     volatile int* info = reinterpret_cast<volatile int*>(tmem_slot + 4);  // lists: the item, for all gather threads
+    int* out_done = reinterpret_cast<int*>(tmem_slot + 12);  // softmax warps through with an item's output
     int* rows_sh = reinterpret_cast<int*>(smem + L::OFF_ROWS);
     volatile int* slots_sh = info;  // dense: first slots of a tile's boxes
 
@@ -391,13 +395,15 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
     if (tid == 0) {
         for (int b = 0; b < 2 * TA_NBUF; ++b) {
             mbar_init(kfull + b, SEL ? L::LOADERS : 1);
-            mbar_init(kfree + b, 1);  // the P.V commit of that half; the MMA warp for a query entry
+            mbar_init(kfree + b, 1);  // the P.V commit of that half; the MMA warp for a query
+                                      // entry, the softmax warps for an item's last tile
         }
         mbar_init(sfull, 1);
         mbar_init(sfull + 1, 1);
         mbar_init(pready, 128);
         mbar_init(pvdone, 1);
         mbar_init(qtmem, 128);
+        *out_done = 0;
         fence_mbar_init();
     }
     if (warp == L::MMA_WARP) tmem_alloc(tmem_slot, 512);
@@ -717,7 +723,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
             __syncwarp();
             return true;
         };
-        auto issue_pv = [&](int entry, int g_, bool first) -> bool {
+        auto issue_pv = [&](int entry, int g_, bool first, bool last) -> bool {
             const int b = entry % TA_NBUF;
             if (!mbar_wait_fast(pready, (uint32_t)g_ & 1u, 54)) return false;
             tc_fence_after();
@@ -729,7 +735,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     for (int ks = 0; ks < TA_TILE / 16; ++ks)
                         mma_bf16(tmem + (uint32_t)(half * 256), p0 + ks * 2, v0 + ((4 * half * L::CHUNK + ks * 2048) >> 4),
                                  L::IDESC_PV, (!first || ks > 0) ? 1u : 0u);
-                    mma_commit(kfree + 2 * b + half);
+                    if (!last) mma_commit(kfree + 2 * b + half);  // the item's last: its output goes through this space
                 }
                 mma_commit(pvdone);
             }
@@ -752,7 +758,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
             if (n > 0) ok = issue_qk(e, gt);
             for (int i = 0; ok && i < n; ++i) {
                 if (i + 1 < n) ok = issue_qk(e + i + 1, gt + i + 1);
-                if (ok) ok = issue_pv(e + i, gt + i, i == 0);
+                if (ok) ok = issue_pv(e + i, gt + i, i == 0, i + 1 == n);
             }
             e += n;
             gt += n;
@@ -763,7 +769,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
         const bool hi_half = lane >= 16;
         const uint32_t lane_o = (uint32_t)(32 * warp) << 16, lane_s = (uint32_t)(32 * warp + 16) << 16;
         int e = 0, gt = 0;
-        int out_row = -1, out_part = -1;  // the item whose output is still in tensor memory
+        int out_row = -1, out_part = -1, out_slot = -1;  // the item whose output is still in tensor memory, its last tile
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
         while (ok) {
@@ -806,55 +812,86 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     if (out_part >= 0) p.lse_part[(long long)out_part * AT_H + h] = lse;
                     else if (p.lse) p.lse[(long long)out_row * AT_H + h] = lse;
                 }
-                // O leaves straight from registers in the fragment shape: four threads write whole 32-byte
-                // sectors of a head's row, and nothing waits (staging through shared memory or every thread
-                // storing its own run of columns took 7,000 and 11,000 cycles an item).
-                const long long at = (out_part >= 0 ? (long long)out_part : (long long)out_row) * AT_H + 16 * warp + (lane >> 2);
-                const float inv0 = __shfl_sync(0xffffffffu, inv, lane >> 2), inv1 = __shfl_sync(0xffffffffu, inv, (lane >> 2) + 8);
-                // an empty row (l = 0) has inv 0, but its O may hold anything
-                const bool any0 = __shfl_sync(0xffffffffu, (int)any, lane >> 2), any1 = __shfl_sync(0xffffffffu, (int)any, (lane >> 2) + 8);
-                const bool narrow = out_part < 0 && p.ctx_bf16;
-                float* of = (out_part >= 0 ? p.o_part : static_cast<float*>(p.ctx)) + at * AT_DV + 2 * (lane & 3);
-                const bool odd = lane & 1;
-                __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(p.ctx) + at * AT_DV + (odd ? 8 : 0) + 4 * ((lane & 3) >> 1);
+                if (!hi_half) {
+                    if (out_part >= 0) p.lse_part[(long long)out_part * AT_H + h] = lse;
+                    else if (p.lse) p.lse[(long long)out_row * AT_H + h] = lse;
+                }
+                if (out_slot >= 0) {
+                    // O leaves through the space of the item's last tile (its P.V is done; the MMA warp leaves it
+                    // to this role to give back), a warp's 16 heads in boxes of 128 bytes a head, by TMA stores:
+                    // nothing waits until the eighth box (stores of single threads took 6,000 to 11,000 cycles).
+                    const bool narrow = out_part < 0 && p.ctx_bf16;
+                    const int y = (out_part >= 0 ? out_part : out_row) * AT_H + 16 * warp;
+                    const uint32_t base = sK + out_slot * L::TILE + warp * 16384u, mine = base + (uint32_t)(lane & 15) * 128u;
+                    auto piece = [&](uint32_t box, int seg, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+                        sts_v4(mine + box * 2048u + (uint32_t)((seg ^ lane) & 7) * 16u, make_uint4(a, b, c, d));
+                    };
 #pragma unroll 1
-                for (int c = 0; c < AT_DV; c += 64) {
-                    float ov[32];
-                    tmem_ld16x256_8(tmem + lane_o + (uint32_t)c, ov);
+                    for (int c = 0; c < AT_DV / 64; ++c) {
+                        float ov[32];
+                        tmem_ld16x2_32<32>(tmem + lane_o + (uint32_t)(64 * c), ov);
 #pragma unroll
-                    for (int x = 0; x < 32; x += 4) {
-                        ov[x] = any0 ? ov[x] * inv0 : 0.f;
-                        ov[x + 1] = any0 ? ov[x + 1] * inv0 : 0.f;
-                        ov[x + 2] = any1 ? ov[x + 2] * inv1 : 0.f;
-                        ov[x + 3] = any1 ? ov[x + 3] * inv1 : 0.f;
-                    }
-                    if (narrow) {
-                        // two groups of 8 columns at a time: neighbours trade, so that an even thread has four
-                        // consecutive columns of the first group and an odd one of the second
+                        for (int x = 0; x < 32; ++x) ov[x] = any ? ov[x] * inv : 0.f;
+                        if (narrow) {
 #pragma unroll
-                        for (int x = 0; x < 32; x += 8) {
+                            for (int k = 0; k < 4; ++k) {
+                                uint32_t w[4];
 #pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                const __nv_bfloat162 f0 = __floats2bfloat162_rn(ov[x + 2 * half], ov[x + 2 * half + 1]);
-                                const __nv_bfloat162 f1 = __floats2bfloat162_rn(ov[x + 4 + 2 * half], ov[x + 5 + 2 * half]);
-                                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(&f0), w1 = *reinterpret_cast<const uint32_t*>(&f1);
-                                const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? w0 : w1, 1);
-                                *reinterpret_cast<uint2*>(ob + half * 8 * AT_DV + c + 2 * x) = odd ? make_uint2(got, w1) : make_uint2(w0, got);
+                                for (int x = 0; x < 4; ++x) {
+                                    const __nv_bfloat162 b2 = __floats2bfloat162_rn(ov[8 * k + 2 * x], ov[8 * k + 2 * x + 1]);
+                                    w[x] = *reinterpret_cast<const uint32_t*>(&b2);
+                                }
+                                piece(c, (hi_half ? 4 : 0) + k, w[0], w[1], w[2], w[3]);
                             }
-                        }
-                    } else {
+                        } else {
+                            if (c >= 4) {  // the eight boxes come round again: their last stores have been read
+                                if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory");
+                                __syncwarp();
+                            }
 #pragma unroll
-                        for (int x = 0; x < 32; x += 4) {
-                            *reinterpret_cast<float2*>(of + c + 2 * x) = make_float2(ov[x], ov[x + 1]);
-                            *reinterpret_cast<float2*>(of + 8 * AT_DV + c + 2 * x) = make_float2(ov[x + 2], ov[x + 3]);
+                            for (int k = 0; k < 8; ++k)
+                                piece((2 * c + (hi_half ? 1 : 0)) & 7, k, __float_as_uint(ov[4 * k]), __float_as_uint(ov[4 * k + 1]),
+                                      __float_as_uint(ov[4 * k + 2]), __float_as_uint(ov[4 * k + 3]));
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (elect_one()) {
+                            if (narrow) {
+                                tma_store2d(&tm.out, 64 * c, y, base + c * 2048u);
+                            } else {
+                                const CUtensorMap* m = out_part >= 0 ? &tm.part : &tm.out;
+                                tma_store2d(m, 64 * c, y, base + ((2 * c) & 7) * 2048u);
+                                tma_store2d(m, 64 * c + 32, y, base + ((2 * c + 1) & 7) * 2048u);
+                            }
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
                     }
+                    if (elect_one()) {
+                        // the copies have read the space; the writes themselves complete with the grid
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __threadfence_block();
+                        if (atomicAdd(out_done, 1) == 3) {  // the last of the four warps gives the space back
+                            *out_done = 0;
+                            mbar_arrive(kfree + 2 * out_slot);
+                            mbar_arrive(kfree + 2 * out_slot + 1);
+                        }
+                    }
+                    __syncwarp();
+                } else {
+                    // an item without a tile: a row that sees nothing, or a run behind a short list's end
+                    const long long at = (out_part >= 0 ? (long long)out_part : (long long)out_row) * AT_H + h;
+                    const bool narrow = out_part < 0 && p.ctx_bf16;
+                    const int n4 = narrow ? AT_DV / 16 : AT_DV / 8;  // 16-byte pieces of half a row
+                    uint4* z = narrow ? reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.ctx) + at * AT_DV)
+                                      : reinterpret_cast<uint4*>((out_part >= 0 ? p.o_part : static_cast<float*>(p.ctx)) + at * AT_DV);
+                    for (int x = 0; x < n4; ++x) z[x + (hi_half ? n4 : 0)] = make_uint4(0, 0, 0, 0);
                 }
                 tc_fence_before();  // these reads come before the next P.V (ordered by pready)
             }
             if (t.x < 0) break;
             out_row = t.x;
             out_part = t.z;
+            out_slot = t.y > 0 ? (e + t.y - 1) % TA_NBUF : -1;
             m_run = -INFINITY;
             l_run = 0.f;
             for (int i = 0; i < t.y && ok; ++i, ++e, ++gt) {

@@ -284,6 +284,25 @@ int encode_o_map(CUtensorMap* tm, void* o_part, int64_t n_parts) {
     return r == CUDA_SUCCESS ? WL_OK : WL_ERR_CUDA;
 }
 
+// A contiguous output [n][64][512], fp32 or bf16, in boxes of 128 bytes x 16 rows, 128B swizzle.
+int encode_out_map(CUtensorMap* tm, void* out, int64_t n, bool bf16) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return WL_ERR_CUDA;
+    const int size = bf16 ? 2 : 4;
+    const cuuint64_t dims[2] = {(cuuint64_t)wl::AT_DV, (cuuint64_t)(wl::AT_H * n)};
+    const cuuint64_t strides[1] = {(cuuint64_t)(wl::AT_DV * size)};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), 16};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, out, dims,
+                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        std::fprintf(stderr, "wl_attn: cuTensorMapEncodeTiled (outputs) failed (%d)\n", (int)r);
+        return WL_ERR_CUDA;
+    }
+    return WL_OK;
+}
+
 int rows_ok(const wl_rows* r, int32_t T) {
     if (!r || r->n_rows <= 0 || r->rows_per_seq <= 0 || r->len0 < 0 || r->len_step < 0 || T <= 0)
         return WL_ERR_ARG;
@@ -1391,6 +1410,8 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     p.box_rows = (kv.page_size & -kv.page_size) < wl::TA_TILE ? (kv.page_size & -kv.page_size) : wl::TA_TILE;
     wl::TreeMaps tm{};
     if (int e = encode_q_map(&tm.q, io->q_abs, io->n_nodes)) return e;
+    if (int e = encode_out_map(&tm.part, p.o_part, parts, false)) return e;
+    if (int e = encode_out_map(&tm.out, io->ctx, io->n_nodes, p.ctx_bf16)) return e;
     const uint64_t slots = (uint64_t)kv.n_pages * kv.page_size;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p.sel) {
