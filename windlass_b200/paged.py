@@ -19,6 +19,7 @@ decodes one sequence, one token at a time, greedily).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -52,25 +53,15 @@ def _table(t: torch.Tensor, batch: int, dev: torch.device) -> int:
     return t.data_ptr()
 
 
-class _On:
-    """The device of a call made current (as torch's own operators do), and its stream."""
-
-    def __init__(self, dev: torch.device):
-        if dev.type != "cuda":
-            raise ValueError(f"tensors must be CUDA tensors, got {dev}")
-        self.dev = dev
-        self.back = None
-
-    def __enter__(self) -> int:
-        cur = torch.cuda.current_device()
-        if cur != self.dev.index:
-            self.back = cur
-            torch.cuda.set_device(self.dev.index)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
+def _call(dev: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` on the current stream of ``dev``, with that device current (as torch's
+    own operators do)."""
+    if dev.type != "cuda":
+        raise ValueError(f"tensors must be CUDA tensors, got {dev}")
+    if torch._C._cuda_getDevice() == dev.index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
 @dataclass
@@ -125,20 +116,23 @@ def page_plan(ctx_len: torch.Tensor, n_new: torch.Tensor, block_table: torch.Ten
     n_free [1] after the call: new tensors, or the given ones with ``in_place``."""
     dev = ctx_len.device
     B, T = ctx_len.numel(), int(n_tokens)
-    out = torch.empty(3 * T + 2 * B + 1, dtype=_I32, device=dev)
-    held_out, free_out = (n_held, n_free) if in_place else (torch.empty_like(n_held), torch.empty_like(n_free))
-    slot, pos, seq = out[:T], out[T:2 * T], out[2 * T:3 * T]
-    cu, short = out[3 * T:3 * T + B + 1], out[3 * T + B + 1:]
-    base = out.data_ptr()
-    io = _lib.PagePlanIO(B, T, page_size, free_list.numel(), _i32(ctx_len, "ctx_len", dev),
-                         _i32(n_new, "n_new", dev, B), _table(block_table, B, dev),
-                         block_table.stride(0) if B > 1 else max(block_table.shape[1], 1), block_table.shape[1],
-                         _i32(n_held, "n_held", dev, B), held_out.data_ptr(), _i32(free_list, "free_list", dev),
-                         _i32(n_free, "n_free", dev, 1), free_out.data_ptr(), base + 12 * T,
-                         base + 4 * (3 * T + B + 1), base, base + 4 * T, base + 8 * T)
-    with _On(dev) as stream:
-        check(lib().wl_page_plan(C.byref(io), stream), "wl_page_plan")
-    return dict(slot=slot, pos=pos, seq=seq, cu=cu, short=short, n_held=held_out, n_free=free_out)
+    c, n, held, nf = (_i32(ctx_len, "ctx_len", dev), _i32(n_new, "n_new", dev, B), _i32(n_held, "n_held", dev, B),
+                      _i32(n_free, "n_free", dev, 1))
+    table, free = _table(block_table, B, dev), _i32(free_list, "free_list", dev)
+    if T < 0:
+        raise ValueError("n_tokens must not be negative")
+    # one allocation: slot, pos, seq [T], cu [B + 1], short [B] and, unless in place, n_held [B] and n_free [1]
+    sizes = [T, T, T, B + 1, B] if in_place else [T, T, T, B + 1, B, B, 1]
+    out = torch.empty(sum(sizes), dtype=_I32, device=dev)
+    o = out.data_ptr()
+    short = o + 4 * (3 * T + B + 1)
+    io = _lib.PagePlanIO(B, T, page_size, free_list.numel(), c, n, table, block_table.stride(0) if B > 1 else max(block_table.shape[1], 1),
+                         block_table.shape[1], held, held if in_place else short + 4 * B, free, nf,
+                         nf if in_place else short + 8 * B, o + 12 * T, short, o, o + 4 * T, o + 8 * T)
+    check(_call(dev, lib().wl_page_plan, C.byref(io)), "wl_page_plan")
+    parts = out.split_with_sizes(sizes)
+    return dict(slot=parts[0], pos=parts[1], seq=parts[2], cu=parts[3], short=parts[4],
+                n_held=n_held if in_place else parts[5], n_free=n_free if in_place else parts[6])
 
 
 def page_release(done: torch.Tensor, block_table: torch.Tensor, n_held: torch.Tensor, free_list: torch.Tensor,
@@ -151,8 +145,7 @@ def page_release(done: torch.Tensor, block_table: torch.Tensor, n_held: torch.Te
             block_table.stride(0) if B > 1 else max(block_table.shape[1], 1), block_table.shape[1],
             _i32(n_held, "n_held", dev, B), _i32(free_list, "free_list", dev), free_list.numel(),
             _i32(n_free, "n_free", dev, 1))
-    with _On(dev) as stream:
-        check(lib().wl_page_release(*args, stream), "wl_page_release")
+    check(_call(dev, lib().wl_page_release, *args), "wl_page_release")
 
 
 def cache_append_paged(cfg: AttnCfg, slot: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
@@ -167,8 +160,7 @@ def cache_append_paged(cfg: AttnCfg, slot: torch.Tensor, cos: torch.Tensor, sin:
         raise ValueError("index pools must be [slots, 128] with scales [slots]")
     io, hold = cache_append_io(slot, cos, sin, kv=None if kv is None else kv.latent(), keys=keys, **kw)
     n_slots = min(t.shape[0] for t in pools)
-    with _On(pools[0].device) as stream:
-        check(lib().wl_cache_append_paged(C.byref(cfg), C.byref(io), n_slots, stream), "wl_cache_append_paged")
+    check(_call(pools[0].device, lib().wl_cache_append_paged, C.byref(cfg), C.byref(io), n_slots), "wl_cache_append_paged")
 
 
 # ---- attention of drafted trees ------------------------------------------------------------------
@@ -229,11 +221,15 @@ def mla_tree_attn(cfg: AttnCfg, kv: PagedKV, q_abs: torch.Tensor, ctx_len: torch
     io = _lib.TreeAttnIO(B, n, _i32(ctx_len, "ctx_len", dev), _i32(cu_nodes, "cu_nodes", dev, B + 1), m, par, kv.c(),
                          q_abs.data_ptr(), mode, _lib.WL_BF16 if out_dtype == torch.bfloat16 else _lib.WL_F32, sel, seln,
                          k, stride, ctx.data_ptr(), lse.data_ptr())
-    L = lib()
-    ws = torch.empty(max(1, L.wl_tree_attn_workspace_bytes(C.byref(cfg), B, n)), dtype=torch.uint8, device=dev)
-    with _On(dev) as stream:
-        check(L.wl_mla_tree_attn(C.byref(cfg), C.byref(io), ws.data_ptr(), ws.numel(), stream), "wl_mla_tree_attn")
+    L, nbytes = lib(), _tree_workspace(B, n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    check(_call(dev, L.wl_mla_tree_attn, C.byref(cfg), C.byref(io), ws.data_ptr(), nbytes), "wl_mla_tree_attn")
     return dict(ctx=ctx, lse=lse)
+
+
+@functools.lru_cache(maxsize=None)
+def _tree_workspace(batch: int, n: int) -> int:
+    return max(1, lib().wl_tree_attn_workspace_bytes(C.byref(_default_cfg()), batch, n))
 
 
 # ---- the commit ----------------------------------------------------------------------------------
@@ -289,17 +285,17 @@ def tree_commit(layers: LayerCaches, ctx_len: torch.Tensor, cu_nodes: torch.Tens
         raise ValueError(f"ctx_len must be on {first.c_kv.device}, got {dev}")
     if first.block_table.shape[0] < B:
         raise ValueError(f"block_table must have {B} rows")
+    sizes = [TREE_MAX * B, B, B, B]
     out = torch.empty((TREE_MAX + 3) * B, dtype=_I32, device=dev)
-    path, acc = out[:TREE_MAX * B].view(B, TREE_MAX), out[TREE_MAX * B:]
-    base = out.data_ptr() + 4 * TREE_MAX * B
+    path = out.data_ptr()
+    acc = path + 4 * TREE_MAX * B
     io = _lib.TreeCommitIO(B, n, _i32(ctx_len, "ctx_len", dev), _i32(cu_nodes, "cu_nodes", dev, B + 1),
                            _i32(parent, "parent", dev), _i32(draft, "draft", dev, n), _i32(target, "target", dev, n),
                            kv.page_size, layers.n_pages, kv.block_table, kv.table_stride, kv.max_pages,
-                           len(layers.kvs), layers._latent, layers._index, base, out.data_ptr(), base + 4 * B,
-                           base + 8 * B)
-    with _On(dev) as stream:
-        check(lib().wl_tree_commit(C.byref(cfg if cfg is not None else _default_cfg()), C.byref(io), stream), "wl_tree_commit")
-    return dict(n_accept=acc[:B], path=path, next=acc[B:2 * B], ctx_len=acc[2 * B:])
+                           len(layers.kvs), layers._latent, layers._index, acc, path, acc + 4 * B, acc + 8 * B)
+    check(_call(dev, lib().wl_tree_commit, C.byref(cfg if cfg is not None else _default_cfg()), C.byref(io)), "wl_tree_commit")
+    parts = out.split_with_sizes(sizes)
+    return dict(n_accept=parts[1], path=parts[0].view(B, TREE_MAX), next=parts[2], ctx_len=parts[3])
 
 
 _cfg: AttnCfg | None = None
