@@ -125,8 +125,12 @@ constexpr int TA_SCHED_THREADS = 192;
 constexpr int TA_MAX_BATCH = 16384;   // the schedule's table of a CTA (8 bytes a request) fits the key tiles' space
 constexpr int TA_CANDS = 64;          // candidate splits: 1..32, then 36, 40, .. 160 (3 x TA_CANDS threads sum up)
 constexpr int TA_MAX_SPLIT = 160;
-constexpr float TA_ITEM_COST = 3.f;   // an item's fixed cost (query in, output out, pipeline fill), in key tiles
-constexpr float TA_PART_COST = 0.04f; // a partial written and joined, in key tiles of one CTA
+// Costs in key tiles of one CTA (1.25 us): an item's query, output and pipeline fill; a partial written and
+// joined, and one beyond a round of the CTAs. Fitted on 16 workloads of 1 to 230 nodes: the second price keeps
+// 15 requests x 4-8 nodes x 2.6K keys whole (64.6 us, 78.2 in runs) and 8 x 18-35 x 4.2K (117 us, 177 in runs),
+// the first, lower one lets 20 nodes x 4K be cut (31.4 us; 36.1 at 0.15).
+constexpr float TA_ITEM_COST = 4.f;
+constexpr float TA_PART_COST = 0.04f, TA_MORE_COST = 0.08f;
 
 template <bool SEL>
 struct TaLayout {
@@ -233,7 +237,8 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
     for (int c = lane; c < TA_CANDS; c += 32) {
         const int n_parts = acc->parts[0][c] + acc->parts[1][c] + acc->parts[2][c];
         const float cost = (acc->sum[0][c] + acc->sum[1][c] + acc->sum[2][c]) * inv_g +
-                           fmaxf(fmaxf(acc->last[0][c], acc->last[1][c]), acc->last[2][c]) + (float)n_parts * TA_PART_COST;
+                           fmaxf(fmaxf(acc->last[0][c], acc->last[1][c]), acc->last[2][c]) + (float)n_parts * TA_PART_COST +
+                           (float)max(0, n_parts - G) * (TA_MORE_COST - TA_PART_COST);
         if (n_parts <= p.parts_max && cost < best) {
             best = cost;
             best_s = tree_candidate(c);
