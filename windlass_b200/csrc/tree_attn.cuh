@@ -129,8 +129,10 @@ constexpr int TA_MAX_SPLIT = 160;
 // joined, and one beyond a round of the CTAs. Fitted on 16 workloads of 1 to 230 nodes: the second price keeps
 // 15 requests x 4-8 nodes x 2.6K keys whole (64.6 us, 78.2 in runs) and 8 x 18-35 x 4.2K (117 us, 177 in runs),
 // the first, lower one lets 20 nodes x 4K be cut (31.4 us; 36.1 at 0.15).
-constexpr float TA_ITEM_COST = 4.f;
-constexpr float TA_PART_COST = 0.04f, TA_MORE_COST = 0.08f;
+struct TreePrice {
+    float item, part, more;
+};
+constexpr TreePrice TA_PRICE = {4.f, 0.04f, 0.08f};
 
 template <bool SEL>
 struct TaLayout {
@@ -191,8 +193,9 @@ struct TreeCost {
 };
 __device__ __forceinline__ int tree_candidate(int c) { return c < 32 ? c + 1 : 32 + 4 * (c - 31); }
 
-__device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* tab, int longest, TreeCost* acc) {
-    const int cand = threadIdx.x % TA_CANDS, grp = threadIdx.x / TA_CANDS, G = gridDim.x;
+template <int PER>  // nodes an item takes
+__device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* tab, int longest, TreeCost* acc, int G, TreePrice price) {
+    const int cand = threadIdx.x % TA_CANDS, grp = threadIdx.x / TA_CANDS;
     const int per = (p.batch + 2) / 3, b0 = min(grp * per, p.batch), b1 = min(b0 + per, p.batch);
     const int s = tree_candidate(cand), C = max(1, div_near(longest + s - 1, s, __fdividef(1.f, (float)s)));
     const float inv = __fdividef(1.f, (float)C);
@@ -203,7 +206,7 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
         for (int b = b0; b < b1; ++b) {
             const int2 v = tab[b];
             const int r = div_near(v.y + C - 1, C, inv);
-            items += v.x * r;
+            items += (v.x + PER - 1) / PER * r;
             parts += r > 1 ? v.x * r : 0;
         }
         acc->items[grp][cand] = items;
@@ -217,9 +220,9 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
 #pragma unroll 2
         for (int b = b0; b < b1; ++b) {
             const int2 v = tab[b];
-            const int r = div_near(v.y + C - 1, C, inv), it = v.x * r;
+            const int r = div_near(v.y + C - 1, C, inv), it = (v.x + PER - 1) / PER * r;
             if (it == 0) continue;
-            const float len = __fdividef((float)v.y, (float)r) + TA_ITEM_COST;
+            const float len = __fdividef((float)v.y, (float)r) + price.item;
             sum += (float)max(0, min(it, full - seen)) * len;
             seen += it;
             if (seen > full) last = fmaxf(last, len);
@@ -237,8 +240,8 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
     for (int c = lane; c < TA_CANDS; c += 32) {
         const int n_parts = acc->parts[0][c] + acc->parts[1][c] + acc->parts[2][c];
         const float cost = (acc->sum[0][c] + acc->sum[1][c] + acc->sum[2][c]) * inv_g +
-                           fmaxf(fmaxf(acc->last[0][c], acc->last[1][c]), acc->last[2][c]) + (float)n_parts * TA_PART_COST +
-                           (float)max(0, n_parts - G) * (TA_MORE_COST - TA_PART_COST);
+                           fmaxf(fmaxf(acc->last[0][c], acc->last[1][c]), acc->last[2][c]) + (float)n_parts * price.part +
+                           (float)max(0, n_parts - G * PER) * (price.more - price.part);
         if (n_parts <= p.parts_max && cost < best) {
             best = cost;
             best_s = tree_candidate(c);
@@ -255,15 +258,13 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
     }
     return max(1, div_near(longest + best_s - 1, best_s, __fdividef(1.f, (float)best_s)));
 }
-// A CTA's item of round k: the CTAs take them forth and back.
-__device__ __forceinline__ int item_of(int k) {
-    return k * (int)gridDim.x + ((k & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
-}
+// Worker me's item of round k: the G workers take them forth and back.
+__device__ __forceinline__ int item_of(int k, int me, int G) { return k * G + ((k & 1) ? G - 1 - me : me); }
 
 
 // Walks the requests with a warp, 32 at a time, and finds the item with a given
 // number (ascending from call to call).
-template <bool SEL>
+template <bool SEL, int PER = 1>
 struct TreeWalk {
     int C, b0, item0, part0;             // block of 32 requests: its first, and the items and parts before it
     int items, parts;                    // of the block
@@ -302,7 +303,7 @@ struct TreeWalk {
         const int r = div_near(tiles + C - 1, C, __fdividef(1.f, (float)C));
         len = r > 1 ? div_near(tiles + r - 1, r, __fdividef(1.f, (float)r)) : max(tiles, 1);
         runs = div_near(tiles + len - 1, len, __fdividef(1.f, (float)len));  // <= r: no run is empty
-        const int it = n * runs, pt = runs > 1 ? it : 0;
+        const int it = (n + PER - 1) / PER * runs, pt = runs > 1 ? n * runs : 0;
         int si = it, sp = pt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -327,12 +328,23 @@ struct TreeWalk {
         return true;
     }
 };
+// The parts of every node, for the merge; by a warp.
+template <bool SEL, int PER>
+__device__ void tree_table(const TreeParams& p, TreeWalk<SEL, PER> w) {
+    for (int r = threadIdx.x & 31; r < p.n_nodes; r += 32) p.node_tab[r] = make_int2(0, 0);
+    __syncwarp();
+    do {
+        if (w.runs > 1)
+            for (int j = 0; j < w.n; ++j) p.node_tab[w.r0 + j] = make_int2(w.part0 + w.excl_part + j * w.runs, w.runs);
+    } while (w.next_block(p));
+}
 struct TreeItem {
     int b, r0, n, ctx, node, tile0, tiles;  // tiles of this item
     int part;                               // -1: the node's only item
+    int runs;
 };
-template <bool SEL>
-__device__ bool tree_item(const TreeParams& p, TreeWalk<SEL>& w, int item, TreeItem& t) {
+template <bool SEL, int PER>
+__device__ bool tree_item(const TreeParams& p, TreeWalk<SEL, PER>& w, int item, TreeItem& t) {
     while (item >= w.item0 + w.items)
         if (!w.next_block(p)) return false;
     const unsigned here = __ballot_sync(0xffffffffu, w.item0 + w.excl_item <= item && w.n * w.runs > 0);
@@ -344,13 +356,69 @@ __device__ bool tree_item(const TreeParams& p, TreeWalk<SEL>& w, int item, TreeI
     t.ctx = __shfl_sync(0xffffffffu, w.ctx, l);
     const int all = __shfl_sync(0xffffffffu, w.tiles, l), runs = __shfl_sync(0xffffffffu, w.runs, l);
     const int len = __shfl_sync(0xffffffffu, w.len, l);
-    const int run = local / t.n;  // the request's nodes side by side on one run of keys
-    t.node = local - run * t.n;
+    const int per = (t.n + PER - 1) / PER;
+    const int run = local / per;  // the request's nodes side by side on one run of keys
+    t.node = (local - run * per) * PER;
     t.tile0 = run * len;
     t.tiles = min(len, all - t.tile0);
+    t.runs = runs;
     t.part = runs > 1 ? w.part0 + __shfl_sync(0xffffffffu, w.excl_part, l) + t.node * runs + run : -1;
     return true;
 }
+
+// The keys of the tile at position pos0 that a node with mask `see` sees.
+__device__ __forceinline__ unsigned long long tree_tile_mask(unsigned long long see, int pos0, int ctx) {
+    if (pos0 + TA_TILE <= ctx) return ~0ull;
+    const int first = pos0 - ctx;  // the tile's first key as a node number
+    return first >= 64 ? 0ull : first >= 0 ? see >> first : (see << -first) | ((1ull << -first) - 1);
+}
+// This lane's box of a run of key tiles (a warp holds the nbox boxes of a tile): its page, loaded a tile ahead,
+// and its first row there; a tile on is `hop` pages and `rest` rows on.
+struct TreePages {
+    const int* table;
+    int nbox, page_size, n_pages, end, hop, rest;
+    int pos, at, off, page;
+    bool mine;
+    __device__ void start(const TreeParams& p, const TreeItem& t) {
+        const int lane = threadIdx.x & 31, R = p.box_rows;
+        table = p.table + (long long)t.b * p.table_stride;
+        nbox = TA_TILE / R;
+        page_size = p.page_size;
+        n_pages = p.n_pages;
+        end = t.ctx + t.n;
+        hop = TA_TILE / page_size;
+        rest = TA_TILE % page_size;
+        pos = t.tile0 * TA_TILE + lane * R;
+        at = pos / page_size;
+        off = pos - at * page_size;
+        mine = lane < nbox && pos < end;
+        page = mine ? __ldg(table + at) : 0;
+    }
+    // First slot of this lane's box of the current tile, behind the pool (read as zeros) past the request's rows
+    // or for a page outside the pool (the error word, and `lost` then holds the tile's keys there), then a tile on.
+    __device__ int next(bool more, unsigned long long& lost) {
+        const bool bad = mine && (page < 0 || page >= n_pages);
+        if (bad) set_error(ERRC_BOUNDS, 46);
+        const int slot = mine && !bad ? page * page_size + off : n_pages * page_size;
+        pos += TA_TILE;
+        at += hop;
+        off += rest;
+        if (off >= page_size) {
+            off -= page_size;
+            ++at;
+        }
+        mine = (int)(threadIdx.x & 31) < nbox && pos < end;
+        if (mine && more) page = __ldg(table + at);
+        lost = 0;
+        const unsigned out = __ballot_sync(0xffffffffu, bad);
+        if (out) {
+            const int R = TA_TILE / nbox;
+            for (int j = 0; j < nbox; ++j)
+                if ((out >> j) & 1) lost |= (R >= 64 ? ~0ull : (1ull << R) - 1) << (j * R);
+        }
+        return slot;
+    }
+};
 
 // One half of a key tile (columns 0-255 and the roped ones, or 256-511) in NB
 // boxes, by one thread: column by column, the boxes' rows in registers. A TMA
@@ -448,7 +516,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
         }
     }
     __syncthreads();
-    walk.C = tree_schedule(p, tab, *longest_sh, cost);
+    walk.C = tree_schedule<1>(p, tab, *longest_sh, cost, gridDim.x, TA_PRICE);
     if (many) {
         fence_proxy_async_smem();  // the table becomes key tiles: its generic accesses come before TMA writes
         __syncthreads();
@@ -456,15 +524,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
 
     if (warp == TA_LOAD_WARP) {  // the producer, or the first gather warp
         walk.count();
-        if (blockIdx.x == gridDim.x - 1) {  // the parts of every node, for the merge
-            for (int r = lane; r < p.n_nodes; r += 32) p.node_tab[r] = make_int2(0, 0);
-            __syncwarp();
-            TreeWalk<SEL> w = walk;
-            do {
-                if (w.runs > 1)
-                    for (int j = 0; j < w.n; ++j) p.node_tab[w.r0 + j] = make_int2(w.part0 + w.excl_part + j * w.runs, w.runs);
-            } while (w.next_block(p));
-        }
+        if (blockIdx.x == gridDim.x - 1) tree_table(p, walk);
     }
 
     if (warp >= TA_LOAD_WARP && warp < L::MMA_WARP) {
@@ -478,7 +538,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
             };
             for (int k = 0; ok; ++k) {
                 TreeItem t{};
-                const bool more = tree_item<SEL>(p, walk, item_of(k), t);
+                const bool more = tree_item(p, walk, item_of(k, blockIdx.x, gridDim.x), t);
                 const int row = t.r0 + t.node, n_tiles = t.tiles;
                 if (!(ok = acquire(0) && acquire(1))) break;
                 {
@@ -501,39 +561,15 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     if (!more) break;
                     ++e;
                 }
-                const int* table = p.table + (long long)t.b * p.table_stride;
-                const int R = p.box_rows, nbox = TA_TILE / R;
-                // this lane's box of a tile: its page (loaded a tile ahead) and its first row there; a tile on is
-                // `hop` pages and `rest` rows on
-                const int hop = TA_TILE / p.page_size, rest = TA_TILE % p.page_size, end = t.ctx + t.n;
-                int pos = t.tile0 * TA_TILE + lane * R, at = pos / p.page_size, off = pos - at * p.page_size;
-                bool mine = lane < nbox && pos < end;
-                int page = mine ? __ldg(table + at) : 0;
+                TreePages pages;
+                pages.start(p, t);
+                const int nbox = pages.nbox;
                 const unsigned long long see = tree_mask_of(p, t.r0, t.n, t.node);
                 for (int i = 0; i < n_tiles && ok; ++i) {
-                    const int pos0 = (t.tile0 + i) * TA_TILE, b = e % TA_NBUF;
-                    // its first slot; behind the pool (read as zeros) past the request's rows or for a bad page
-                    const bool bad = mine && (page < 0 || page >= p.n_pages);
-                    if (bad) set_error(ERRC_BOUNDS, 46);
-                    const int slot = mine && !bad ? page * p.page_size + off : p.n_pages * p.page_size;
-                    pos += TA_TILE;
-                    at += hop;
-                    off += rest;
-                    if (off >= p.page_size) {
-                        off -= p.page_size;
-                        ++at;
-                    }
-                    mine = lane < nbox && pos < end;
-                    if (mine && i + 1 < n_tiles) page = __ldg(table + at);
-                    const unsigned lost = __ballot_sync(0xffffffffu, bad);
-                    unsigned long long v = ~0ull;
-                    if (pos0 + TA_TILE > t.ctx) {  // drafted rows, or none
-                        const int first = pos0 - t.ctx;  // first key as a node number
-                        v = first >= 64 ? 0ull : first >= 0 ? see >> first : (see << -first) | ((1ull << -first) - 1);
-                    }
-                    if (lost)
-                        for (int j = 0; j < nbox; ++j)
-                            if ((lost >> j) & 1) v &= ~((R >= 64 ? ~0ull : (1ull << R) - 1) << (j * R));
+                    const int b = e % TA_NBUF;
+                    unsigned long long lost;
+                    const int slot = pages.next(i + 1 < n_tiles, lost);
+                    const unsigned long long v = tree_tile_mask(see, (t.tile0 + i) * TA_TILE, t.ctx) & ~lost;
                     if (lane < 8) slots_sh[lane] = slot;
                     if (!(ok = acquire(0))) break;
                     if (lane == 0) see_sh[b] = v;
@@ -590,7 +626,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
             for (int k = 0; ok; ++k) {
                 TreeItem t{};
                 if (warp == TA_LOAD_WARP) {
-                    const bool more = tree_item<SEL>(p, walk, item_of(k), t);
+                    const bool more = tree_item(p, walk, item_of(k, blockIdx.x, gridDim.x), t);
                     unsigned long long see = 0;
                     int left = 0;  // entries of this item
                     if (more) {

@@ -29,6 +29,7 @@
 #include "paged.cuh"
 #include "topk.cuh"
 #include "tree_attn.cuh"
+#include "tree_pair.cuh"
 #include "xmerge.cuh"
 #include "gemv_tc.cuh"
 
@@ -86,11 +87,18 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 std::mutex g_attr_mu;
 bool g_attr_done[kMaxDevices];
 int g_sm_count[kMaxDevices];
+int g_pair_count[kMaxDevices];  // CTA pairs of tree_pair_kernel that run at a time
 
 int sm_count() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
     return g_sm_count[dev] > 0 ? g_sm_count[dev] : 148;
+}
+
+int pair_count() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 1;
+    return g_pair_count[dev] > 0 ? g_pair_count[dev] : 1;
 }
 
 int ensure_attrs() {
@@ -126,6 +134,23 @@ int ensure_attrs() {
     int sms = 0;
     WL_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     g_sm_count[dev] = sms;
+    {
+        WL_CUDA_TRY(cudaFuncSetAttribute(wl::tree_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, wl::TpLayout::BYTES));
+        cudaLaunchConfig_t lc{};
+        lc.gridDim = dim3(sms / 2 * 2);
+        lc.blockDim = dim3(wl::TP_THREADS);
+        lc.dynamicSmemBytes = wl::TpLayout::BYTES;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2;
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        lc.attrs = at;
+        lc.numAttrs = 1;
+        int n = 0;
+        WL_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, wl::tree_pair_kernel, &lc));
+        g_pair_count[dev] = n < sms / 2 ? n : sms / 2;
+    }
     g_attr_done[dev] = true;
     return WL_OK;
 }
@@ -284,14 +309,14 @@ int encode_o_map(CUtensorMap* tm, void* o_part, int64_t n_parts) {
     return r == CUDA_SUCCESS ? WL_OK : WL_ERR_CUDA;
 }
 
-// A contiguous output [n][64][512], fp32 or bf16, in boxes of 128 bytes x 16 rows, 128B swizzle.
-int encode_out_map(CUtensorMap* tm, void* out, int64_t n, bool bf16) {
+// A contiguous output [n][64][512], fp32 or bf16, in boxes of 128 bytes x `rows` rows, 128B swizzle.
+int encode_out_map(CUtensorMap* tm, void* out, int64_t n, bool bf16, uint32_t rows) {
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return WL_ERR_CUDA;
     const int size = bf16 ? 2 : 4;
     const cuuint64_t dims[2] = {(cuuint64_t)wl::AT_DV, (cuuint64_t)(wl::AT_H * n)};
     const cuuint64_t strides[1] = {(cuuint64_t)(wl::AT_DV * size)};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), 16};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), rows};
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, out, dims,
                            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1410,17 +1435,39 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     p.box_rows = (kv.page_size & -kv.page_size) < wl::TA_TILE ? (kv.page_size & -kv.page_size) : wl::TA_TILE;
     wl::TreeMaps tm{};
     if (int e = encode_q_map(&tm.q, io->q_abs, io->n_nodes)) return e;
-    if (int e = encode_out_map(&tm.part, p.o_part, parts, false)) return e;
-    if (int e = encode_out_map(&tm.out, io->ctx, io->n_nodes, p.ctx_bf16)) return e;
+    // Two nodes of a request at a time, by CTA pairs, when requests have two and more on average; one at a time
+    // otherwise (a lone node leaves half of a pair's rows empty), and for lists (a list per node).
+    const bool pairs = !p.sel && 2 * (int64_t)io->n_nodes >= 3 * (int64_t)io->batch;
+    const uint32_t out_rows = pairs ? 32 : 16;  // a warp's rows
+    if (int e = encode_out_map(&tm.part, p.o_part, parts, false, out_rows)) return e;
+    if (int e = encode_out_map(&tm.out, io->ctx, io->n_nodes, p.ctx_bf16, out_rows)) return e;
     const uint64_t slots = (uint64_t)kv.n_pages * kv.page_size;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p.sel) {
-        WL_CUDA_TRY(launch_pdl(wl::tree_attn_kernel<true>, dim3(sm_count()), dim3(wl::TaLayout<true>::THREADS),
-                               wl::TaLayout<true>::BYTES, st, p, tm));
-    } else {
+    if (!p.sel) {
         if (int e = encode_bf16_2d(&tm.ckv, kv.latent.c_kv, wl::AT_DV, slots, kv.latent.c_kv_row_stride, 64, p.box_rows)) return e;
         if (int e = encode_bf16_2d(&tm.krot, kv.latent.k_rot, wl::AT_D - wl::AT_DV, slots, kv.latent.k_rot_row_stride, 64, p.box_rows))
             return e;
+    }
+    if (p.sel) {
+        WL_CUDA_TRY(launch_pdl(wl::tree_attn_kernel<true>, dim3(sm_count()), dim3(wl::TaLayout<true>::THREADS),
+                               wl::TaLayout<true>::BYTES, st, p, tm));
+    } else if (pairs) {
+        cudaLaunchConfig_t lc{};
+        lc.gridDim = dim3(2 * pair_count());
+        lc.blockDim = dim3(wl::TP_THREADS);
+        lc.dynamicSmemBytes = wl::TpLayout::BYTES;
+        lc.stream = st;
+        cudaLaunchAttribute at[2];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2;
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[1].val.programmaticStreamSerializationAllowed = 1;
+        lc.attrs = at;
+        lc.numAttrs = pdl_enabled() ? 2 : 1;
+        WL_CUDA_TRY(cudaLaunchKernelEx(&lc, wl::tree_pair_kernel, p, tm));
+    } else {
         WL_CUDA_TRY(launch_pdl(wl::tree_attn_kernel<false>, dim3(sm_count()), dim3(wl::TaLayout<false>::THREADS),
                                wl::TaLayout<false>::BYTES, st, p, tm));
     }
