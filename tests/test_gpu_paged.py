@@ -259,6 +259,18 @@ def test_many_requests_and_long_contexts():
     t.check(t.call())
 
 
+@pytest.mark.parametrize("B,lo,hi", [(30, 8, 12), (60, 2, 4), (61, 1, 9), (200, 1, 3)])
+def test_more_work_than_a_round_of_the_gpu(B, lo, hi):
+    """Every CTA (pair) takes several pieces of work one after the other, of all lengths."""
+    rng = np.random.default_rng(B)
+    t = Trees(rng.integers(0, 400, B).tolist(), rng.integers(lo, hi, B).tolist(), 16 if B % 2 else 64, seed=B)
+    got = t.call()
+    t.check(got)
+    for _ in range(5):
+        again = t.call()
+        assert torch.equal(again["ctx"], got["ctx"]) and torch.equal(again["lse"], got["lse"])
+
+
 def test_a_node_may_see_other_than_its_ancestors_or_nothing():
     t = Trees([0, 70], [6, 4], 16, seed=6)
     masks = [0, 0b10, 0b111111, 0b000001, 0b100000, 0, 0, 0b1000, 0b1111, 0b0101]

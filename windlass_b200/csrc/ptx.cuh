@@ -272,6 +272,13 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
         }
     }
 }
+// mma_commit on the mbarrier at the same place in every CTA of the cluster named by `ctas` (a bit each).
+__device__ __forceinline__ void mma_commit_cluster(uint64_t* bar, uint16_t ctas) {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"(ctas)
+        : "memory");
+}
 // Bulk copy of this CTA's shared memory into another CTA's, completing on that
 // CTA's mbarrier (dst and bar are dsmem_addr addresses; 16-byte multiples).
 __device__ __forceinline__ void bulk_s2s(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {

@@ -194,7 +194,8 @@ struct TreeCost {
 __device__ __forceinline__ int tree_candidate(int c) { return c < 32 ? c + 1 : 32 + 4 * (c - 31); }
 
 template <int PER>  // nodes an item takes
-__device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* tab, int longest, TreeCost* acc, int G, TreePrice price) {
+__device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* tab, int longest, TreeCost* acc, int G, TreePrice price,
+                                             int last_warp = TA_LOAD_WARP) {
     const int cand = threadIdx.x % TA_CANDS, grp = threadIdx.x / TA_CANDS;
     const int per = (p.batch + 2) / 3, b0 = min(grp * per, p.batch), b1 = min(b0 + per, p.batch);
     const int s = tree_candidate(cand), C = max(1, div_near(longest + s - 1, s, __fdividef(1.f, (float)s)));
@@ -231,7 +232,7 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
         acc->last[grp][cand] = last;
     }
     __syncthreads();
-    if (threadIdx.x / 32 != TA_LOAD_WARP) return 0;
+    if ((int)threadIdx.x / 32 != last_warp) return 0;
     const int lane = threadIdx.x & 31;
     float best = 3e38f;
     int best_s = 1;

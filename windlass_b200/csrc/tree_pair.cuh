@@ -8,9 +8,10 @@
 // of 64 keys:
 //   score CTA  S = Q K^T (A = the queries in tensor memory, 288 columns; S twice
 //              64 columns): 36 MMAs M = 128, N = 64: 1,152 cycles. Its softmax
-//              warps keep the running maximum and sum, one row a thread, and a
-//              bulk copy takes P (bf16, 16 KB) and the rows' rescale factors to
-//              the value CTA's shared memory.
+//              warps keep the running maximum and sum, one row a thread; each
+//              sends its rows' P (bf16, 4 KB) and rescale factors by a bulk copy
+//              into the value CTA's shared memory, four tiles deep (stores of
+//              16 bytes to the other SM took 4,700 cycles a tile).
 //   value CTA  O += P V: 8 MMAs M = 128, N = 256: 1,024 cycles. Four warps rescale
 //              O when a factor is not 1 (rare: the maximum moves only by more than
 //              2^8), and write O / l at the end of an item.
@@ -27,32 +28,40 @@
 
 namespace wl {
 
-constexpr int TP_THREADS = 224;  // warps 0-3 rows, 4 loads, 5 MMA, 6 copies P over (score) / tells of freed P (value)
-constexpr int TP_UNITS = 7;      // score CTA's ring: units of 64 keys x 192 columns (a third of a tile)
-constexpr int TP_VBUF = 3;       // value CTA's ring: tiles of 64 keys x 512 columns, in halves
+// Warps 0-7 rows (score: four for even and four for odd tiles; value: 0-3), 8 and 9 loads of even and odd tiles,
+// 10 and 11 MMAs (score: of even and odd tiles; value: 10). One warp for each took 1,500 to 1,700 cycles a tile.
+constexpr int TP_THREADS = 384;
+constexpr int TP_LOAD_WARP = 8, TP_MMA_WARP = 10;
+// Even and odd tiles have their own space, loader, MMA warp and softmax warps throughout, so that each barrier's
+// phases are waited for one after the other by the same threads (a wait that skipped a phase could take an older
+// one for it):
+constexpr int TP_UNITS = 6;   // score CTA: [even, odd][3] thirds of a tile (64 keys x 192 columns), the queries' way in
+constexpr int TP_HALVES = 4;  // value CTA: [even, odd][2] halves of a tile (64 keys x 256 columns)
+constexpr int TP_P = 4;       // value CTA: tiles of P (score CTA: on their way), tile & 3
 constexpr uint32_t TP_TM_S = 384;  // score columns in tensor memory (the queries take [0, 288))
 constexpr TreePrice TP_PRICE = {9.f, 0.08f, 0.16f};
 
 struct TpLayout {
     static constexpr uint32_t CHUNK = TA_TILE * 128;          // 8 KB: 64 keys x 64 columns
-    static constexpr uint32_t UNIT = 3 * CHUNK, HALF = 4 * CHUNK, VTILE = 2 * HALF;
+    static constexpr uint32_t UNIT = 3 * CHUNK, HALF = 4 * CHUNK;
     static constexpr uint32_t P = 128 * 128;                  // 128 rows x 64 keys bf16
-    static constexpr uint32_t OFF_PS = TP_UNITS * UNIT;       // score CTA: P on its way (two)
-    static constexpr uint32_t OFF_P = TP_VBUF * VTILE;        // value CTA: P arrived (two)
-    static constexpr uint32_t OFF_ALPHA = OFF_P + 2 * P;      // both: rescale factors [2][128]
-    static constexpr uint32_t OFF_FIN = OFF_ALPHA + 1024;     // value CTA: 1 / l of the item's rows [128]
-    static constexpr uint32_t OFF_ITEM = OFF_FIN + 512;       // item descriptors [2]
+    static constexpr uint32_t OFF_P = TP_HALVES * HALF;       // value CTA
+    static constexpr uint32_t OFF_PS = TP_UNITS * UNIT;       // score CTA: P on its way
+    static constexpr uint32_t OFF_ALPHA = OFF_PS + TP_P * P;  // both: rescale factors [TP_P][128]
+    static constexpr uint32_t OFF_FIN = OFF_ALPHA + TP_P * 512;  // value CTA: 1 / l of the item's rows [128]
+    static constexpr uint32_t OFF_MAX = OFF_FIN + 512;        // score CTA: rows' maxima after even and odd tiles [2][128]
+    static constexpr uint32_t OFF_SUM = OFF_MAX + 1024;       // score CTA: one half's (sum, maximum) at an item's end [128]
+    static constexpr uint32_t OFF_ITEM = OFF_SUM + 1024;      // item descriptors [2]
     static constexpr uint32_t OFF_LOST = OFF_ITEM + 128;      // keys lost to bad pages, per tile [8]
     static constexpr uint32_t OFF_BAR = OFF_LOST + 64;
-    static constexpr int N_BARS = 28;
-    static constexpr uint32_t OFF_MISC = OFF_BAR + N_BARS * 8;  // tensor-memory slot, longest, out count, slots [8]
-    static constexpr uint32_t BYTES = OFF_MISC + 48 + 1024;
+    static constexpr int N_BARS = 34;
+    static constexpr uint32_t OFF_MISC = OFF_BAR + N_BARS * 8;  // tensor-memory slot, longest, out count, slots [2][8]
+    static constexpr uint32_t BYTES = OFF_MISC + 80 + 1024;
     static constexpr uint32_t IDESC_QK = idesc_bf16(128, TA_TILE, 0, 0);
     static constexpr uint32_t IDESC_PV = idesc_bf16(128, 256, 0, 1);
-    static constexpr uint32_t COPY = P + 512;
 };
 static_assert(TpLayout::BYTES <= 232448, "one CTA per SM");
-static_assert(TpLayout::OFF_PS + 2 * TpLayout::P <= TpLayout::OFF_ALPHA, "score CTA's layout");
+static_assert(TP_P == 4 && TpLayout::OFF_P + TP_P * TpLayout::P <= TpLayout::OFF_ALPHA, "value CTA's layout");
 
 struct TpItem {  // what the roles of a CTA need of an item
     int rows, row0;        // nodes (1 or 2; 0: no more), first row
@@ -70,28 +79,32 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     return y;
 }
 
-// `count` column chunks from c0 on of a key tile in NB boxes (see tree_boxes).
-template <int NB>
-__device__ __forceinline__ void pair_boxes(const TreeMaps& tm, uint32_t dst, int c0, int count, const volatile int* rows, uint64_t* bar) {
+// N column chunks from C0 on of a key tile in NB boxes, by one thread (see tree_boxes).
+template <int NB, int C0, int N>
+__device__ __forceinline__ void pair_boxes(const TreeMaps& tm, uint32_t dst, const volatile int* rows, uint64_t* bar) {
     constexpr uint32_t CHUNK = TA_TILE * 128, BOX = CHUNK / NB;
+    constexpr int M = C0 + N > 8 ? 8 - C0 : N;  // latent chunks; the ninth is the roped one
     int y[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) y[j] = rows[j];
-#pragma unroll 1
-    for (int c = c0; c < c0 + count; ++c, dst += CHUNK) {
-        const CUtensorMap* m = c < 8 ? &tm.ckv : &tm.krot;
-        const int x = c < 8 ? c * 64 : 0;
+#pragma unroll(NB <= 2 ? 4 : 1)
+    for (int c = 0; c < M; ++c) {
 #pragma unroll
-        for (int j = 0; j < NB; ++j) tma_load2d(dst + j * BOX, m, x, y[j], bar);
+        for (int j = 0; j < NB; ++j) tma_load2d(dst + c * CHUNK + j * BOX, &tm.ckv, (C0 + c) * 64, y[j], bar);
+    }
+    if (M < N) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) tma_load2d(dst + M * CHUNK + j * BOX, &tm.krot, 0, y[j], bar);
     }
 }
-__device__ __forceinline__ void pair_load(const TreeMaps& tm, uint32_t dst, int c0, int count, int nbox, const volatile int* rows, uint64_t* bar) {
+template <int C0, int N>
+__device__ __forceinline__ void pair_load(const TreeMaps& tm, uint32_t dst, int nbox, const volatile int* rows, uint64_t* bar) {
     if (elect_one()) {
-        mbar_expect_tx(bar, (uint32_t)count * TpLayout::CHUNK);
-        if (nbox == 1) pair_boxes<1>(tm, dst, c0, count, rows, bar);
-        else if (nbox == 2) pair_boxes<2>(tm, dst, c0, count, rows, bar);
-        else if (nbox == 4) pair_boxes<4>(tm, dst, c0, count, rows, bar);
-        else pair_boxes<8>(tm, dst, c0, count, rows, bar);
+        mbar_expect_tx(bar, (uint32_t)N * TpLayout::CHUNK);
+        if (nbox == 1) pair_boxes<1, C0, N>(tm, dst, rows, bar);
+        else if (nbox == 2) pair_boxes<2, C0, N>(tm, dst, rows, bar);
+        else if (nbox == 4) pair_boxes<4, C0, N>(tm, dst, rows, bar);
+        else pair_boxes<8, C0, N>(tm, dst, rows, bar);
     }
     __syncwarp();
 }
@@ -109,15 +122,17 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
     const uint32_t base = smem_u32(smem);
     float* alpha_sh = reinterpret_cast<float*>(smem + L::OFF_ALPHA);
     float* fin_sh = reinterpret_cast<float*>(smem + L::OFF_FIN);
+    float* max_sh = reinterpret_cast<float*>(smem + L::OFF_MAX);
+    float2* sum_sh = reinterpret_cast<float2*>(smem + L::OFF_SUM);
     TpItem* item_sh = reinterpret_cast<TpItem*>(smem + L::OFF_ITEM);
     unsigned long long* lost_sh = reinterpret_cast<unsigned long long*>(smem + L::OFF_LOST);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
     uint64_t *ifull = bars, *ifree = bars + 2;  // item descriptors
     // score CTA
-    uint64_t *ufull = bars + 4, *ufree = bars + 11, *qtmem = bars + 18, *sfull = bars + 19, *sfree = bars + 21, *pstaged = bars + 23,
-             *pfree = bars + 25, *finfree = bars + 27;
-    // value CTA
-    uint64_t *vfull = bars + 4, *vfree = bars + 10, *pfull = bars + 16, *pok = bars + 18, *pvdone = bars + 19, *finfull = bars + 21;
+    uint64_t *ufull = bars + 4, *ufree = bars + 10, *qtmem = bars + 16, *sfull = bars + 17, *sfree = bars + 19, *pfree = bars + 21,
+             *finfree = bars + 25, *mready = bars + 26, *lready = bars + 28, *ldone = bars + 29;
+    // value CTA (pfree's places are not used here: the commit that frees P names them in the score CTA)
+    uint64_t *vfull = bars + 4, *vfree = bars + 8, *pfull = bars + 12, *pok = bars + 16, *pvdone = bars + 26, *finfull = bars + 30;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
     int* longest_sh = reinterpret_cast<int*>(tmem_slot + 1);
     int* out_done = reinterpret_cast<int*>(tmem_slot + 2);
@@ -130,40 +145,42 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(ifull + i, 1);
-            mbar_init(ifree + i, 6);  // a lane of each consumer warp
+            mbar_init(ifree + i, score ? 10 : 5);  // a lane of each consumer warp
         }
         if (score) {
             for (int i = 0; i < TP_UNITS; ++i) {
                 mbar_init(ufull + i, 1);
                 mbar_init(ufree + i, 1);
             }
-            mbar_init(qtmem, 128);
+            mbar_init(qtmem, 256);
             for (int i = 0; i < 2; ++i) {
                 mbar_init(sfull + i, 1);
                 mbar_init(sfree + i, 128);
-                mbar_init(pstaged + i, 128);
-                mbar_init(pfree + i, 1);
+                mbar_init(mready + i, 128);
             }
+            mbar_init(lready, 128);
+            mbar_init(ldone, 128);
+            for (int i = 0; i < TP_P; ++i) mbar_init(pfree + i, 1);
             mbar_init(finfree, 4);
         } else {
-            for (int i = 0; i < 2 * TP_VBUF; ++i) {
+            for (int i = 0; i < TP_HALVES; ++i) {
                 mbar_init(vfull + i, 1);
                 mbar_init(vfree + i, 1);
             }
-            mbar_init(pfull, 1);
-            mbar_init(pfull + 1, 1);
-            mbar_init(pok, 128);
-            mbar_init(pvdone, 1);
-            mbar_init(pvdone + 1, 1);
+            for (int i = 0; i < TP_P; ++i) {
+                mbar_init(pfull + i, 1);
+                mbar_init(pok + i, 128);
+                mbar_init(pvdone + i, 1);
+            }
             mbar_init(finfull, 128);
             *out_done = 0;
         }
         fence_mbar_init();
         if (!score)
-            for (int i = 0; i < 2; ++i) mbar_expect_tx(pfull + i, L::COPY);
+            for (int i = 0; i < TP_P; ++i) mbar_expect_tx(pfull + i, L::P + 512);
     }
-    if (warp == 5) tmem_alloc(tmem_slot, 512);
-    if (warp == 4 && lane < 3)
+    if (warp == TP_MMA_WARP) tmem_alloc(tmem_slot, 512);
+    if (warp == TP_LOAD_WARP && lane < 3)
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &tm.q : lane == 1 ? &tm.ckv : &tm.krot)) : "memory");
     tc_fence_before();
     __syncthreads();
@@ -188,19 +205,22 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
         }
         if (longest > 0) atomicMax(longest_sh, longest);
     }
-    if (warp == TA_LOAD_WARP) {
+    const bool loads = warp == TP_LOAD_WARP || warp == TP_LOAD_WARP + 1;
+    if (loads) {
         walk.b0 = walk.item0 = walk.part0 = 0;
         walk.load(p);
         if (!many) {
             if (p.batch > 1) walk.sort();
-            if (lane < p.batch) tab[lane] = make_int2(walk.n, walk.tiles);
-            if (lane == 0) *longest_sh = walk.tiles;
+            if (warp == TP_LOAD_WARP && lane < p.batch) tab[lane] = make_int2(walk.n, walk.tiles);
+            if (warp == TP_LOAD_WARP && lane == 0) *longest_sh = walk.tiles;
         }
     }
     __syncthreads();
-    walk.C = tree_schedule<2>(p, tab, *longest_sh, cost, G, TP_PRICE);
+    const int chosen = tree_schedule<2>(p, tab, *longest_sh, cost, G, TP_PRICE, TP_LOAD_WARP);
+    if (warp == TP_LOAD_WARP && lane == 0) *longest_sh = chosen;
     fence_proxy_async_smem();  // the scratch becomes key tiles and P: its generic accesses come before async writes
     __syncthreads();
+    walk.C = *longest_sh;
 
     bool ok = true;
     // the consumers' view of item k
@@ -212,154 +232,143 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
         if (lane == 0) mbar_arrive(ifree + x);
         return true;
     };
-    if (warp == 4) {
-        // ---------------- loads ----------------
+    if (loads) {
+        // ---------------- loads: even or odd tiles ----------------
         walk.count();
-        if (score && me == G - 1) tree_table(p, walk);
-        int u = 0, round = 0, gt = 0;  // ring unit (score: a third of a tile, value: half) and how often it went round
-        const int ring = score ? TP_UNITS : 2 * TP_VBUF;
-        uint64_t *full = score ? ufull : vfull, *free_ = score ? ufree : vfree;
-        const uint32_t unit = score ? L::UNIT : L::HALF;
-        auto acquire = [&]() -> bool { return round == 0 || mbar_wait_fast(free_ + u, (uint32_t)(round - 1) & 1u, 71); };
-        auto advance = [&]() {
-            if (++u == ring) {
-                u = 0;
-                ++round;
-            }
-        };
+        const int which = warp - TP_LOAD_WARP;
+        if (score && me == G - 1 && which == 0) tree_table(p, walk);
+        const int steps = score ? 3 : 2;          // pieces of a tile
+        const int first = which * steps;          // this loader's barriers
+        int use = 0, gt = 0;                      // times its space was filled; the CTA's tiles so far
+        uint64_t *full = (score ? ufull : vfull) + first, *free_ = (score ? ufree : vfree) + first;
+        volatile int* slots = slots_sh + 8 * which;
+        const uint32_t space = base + (uint32_t)first * (score ? L::UNIT : L::HALF);
+        auto acquire = [&](int j) -> bool { return use == 0 || mbar_wait_fast(free_ + j, (uint32_t)(use - 1) & 1u, 71); };
         for (int k = 0; ok; ++k) {
             TreeItem t{};
             const bool more = tree_item(p, walk, item_of(k, me, G), t);
             const int rows = more ? min(2, t.n - t.node) : 0;
             if (score && more) {
-                // the queries: two nodes x three units (a lone node's twice)
-                for (int q = 0; q < 6 && ok; ++q) {
-                    if (!(ok = acquire())) break;
-                    const int y = (t.r0 + t.node + min(q / 3, rows - 1)) * AT_H;
+                // the query of the first node by the one loader, of the second (a lone node's again) by the other
+                for (int j = 0; j < 3; ++j) {
+                    if (!(ok = acquire(j))) break;
+                    const int y = (t.r0 + t.node + min(which, rows - 1)) * AT_H;
                     if (elect_one()) {
-                        mbar_expect_tx(ufull + u, L::UNIT);
-                        for (int c = 0; c < 3; ++c)
-                            tma_load2d(base + u * L::UNIT + c * L::CHUNK, &tm.q, (3 * (q % 3) + c) * 64, y, ufull + u);
+                        mbar_expect_tx(full + j, L::UNIT);
+                        for (int c = 0; c < 3; ++c) tma_load2d(space + j * L::UNIT + c * L::CHUNK, &tm.q, (3 * j + c) * 64, y, full + j);
                     }
                     __syncwarp();
-                    advance();
                 }
                 if (!ok) break;
+                ++use;
             }
-            if (k >= 2 && !(ok = mbar_wait_fast(ifree + (k & 1), (uint32_t)((k >> 1) - 1) & 1u, 72))) break;
-            TpItem d{};
             TreePages pages;
-            if (more) {
-                pages.start(p, t);
-                d.see[0] = tree_mask_of(p, t.r0, t.n, t.node);
-                d.see[1] = rows > 1 ? tree_mask_of(p, t.r0, t.n, t.node + 1) : d.see[0];
-                d.rows = rows;
-                d.row0 = t.r0 + t.node;
-                d.tiles = t.tiles;
-                d.pos0 = t.tile0 * TA_TILE;
-                d.ctx = t.ctx;
-                d.part = t.part;
-                d.runs = t.runs;
+            if (more) pages.start(p, t);
+            if (which == 0) {
+                if (k >= 2 && !(ok = mbar_wait_fast(ifree + (k & 1), (uint32_t)((k >> 1) - 1) & 1u, 72))) break;
+                TpItem d{};
+                if (more) {
+                    d.see[0] = tree_mask_of(p, t.r0, t.n, t.node);
+                    d.see[1] = rows > 1 ? tree_mask_of(p, t.r0, t.n, t.node + 1) : d.see[0];
+                    d.rows = rows;
+                    d.row0 = t.r0 + t.node;
+                    d.tiles = t.tiles;
+                    d.pos0 = t.tile0 * TA_TILE;
+                    d.ctx = t.ctx;
+                    d.part = t.part;
+                    d.runs = t.runs;
+                }
+                if (lane == 0) {
+                    item_sh[k & 1] = d;
+                    mbar_arrive(ifull + (k & 1));
+                }
+                __syncwarp();
             }
-            if (lane == 0) {
-                item_sh[k & 1] = d;
-                mbar_arrive(ifull + (k & 1));
-            }
-            __syncwarp();
             if (!more) break;
-            for (int i = 0; i < t.tiles && ok; ++i, ++gt) {
+            for (int i = 0; i < t.tiles; ++i, ++gt) {
                 unsigned long long lost;
                 const int slot = pages.next(i + 1 < t.tiles, lost);
-                if (lane < 8) slots_sh[lane] = slot;
+                if ((gt & 1) != which) continue;
+                if (lane < 8) slots[lane] = slot;
                 if (lane == 0) lost_sh[gt & 7] = lost;
                 __syncwarp();
-                const int steps = score ? 3 : 2, width = score ? 3 : 4;
-                for (int j = 0; j < steps; ++j) {
-                    if (!(ok = acquire())) break;
-                    pair_load(tm, base + u * unit, j * width, width, pages.nbox, slots_sh, full + u);
-                    advance();
+                if (score) {
+                    if (!(ok = acquire(0))) break;
+                    pair_load<0, 3>(tm, space, pages.nbox, slots, full);
+                    if (!(ok = acquire(1))) break;
+                    pair_load<3, 3>(tm, space + L::UNIT, pages.nbox, slots, full + 1);
+                    if (!(ok = acquire(2))) break;
+                    pair_load<6, 3>(tm, space + 2 * L::UNIT, pages.nbox, slots, full + 2);
+                } else {
+                    if (!(ok = acquire(0))) break;
+                    pair_load<0, 4>(tm, space, pages.nbox, slots, full);
+                    if (!(ok = acquire(1))) break;
+                    pair_load<4, 4>(tm, space + L::HALF, pages.nbox, slots, full + 1);
                 }
+                ++use;
             }
         }
-        if (!ok)  // copies in flight must land before the CTA leaves
-            for (int i = 0; i < ring; ++i)
-                if (i < u || round > 0) mbar_wait_fast(full + i, (uint32_t)(i < u ? round : round - 1) & 1u, 73);
-    } else if (score && warp == 5) {
-        // ---------------- score CTA: Q K^T ----------------
-        int u = 0, uph = 0, gt = 0;
-        auto advance = [&]() {
-            if (++u == TP_UNITS) {
-                u = 0;
-                uph ^= 1;
-            }
-        };
+        if (!ok && use > 0)  // copies in flight must land before the CTA leaves
+            for (int j = 0; j < steps; ++j) mbar_wait_fast(full + j, (uint32_t)(use - 1) & 1u, 73);
+    } else if (score && warp >= TP_MMA_WARP) {
+        // ---------------- score CTA: Q K^T of even or odd tiles ----------------
+        // (two warps, so that the waits of one tile pass under the MMAs of the other)
+        const int s = warp - TP_MMA_WARP;
+        const uint32_t d = tmem + TP_TM_S + (uint32_t)(s * TA_TILE);
+        uint64_t *full = ufull + 3 * s, *free_ = ufree + 3 * s;
+        const uint64_t k0 = desc_sw128(base + (uint32_t)(3 * s) * L::UNIT, 16, 1024);
+        int use = 0, gt = 0;
         for (int k = 0; ok; ++k) {
             TpItem t;
             if (!(ok = take(k, t)) || t.rows == 0) break;
             if (!(ok = mbar_wait_fast(qtmem, (uint32_t)k & 1u, 74))) break;  // the queries are in tensor memory
-            for (int q = 0; q < 6; ++q) {
-                if (elect_one()) mbar_arrive(ufree + u);
-                advance();
-            }
+            if (elect_one())
+                for (int j = 0; j < 3; ++j) mbar_arrive(free_ + j);
+            __syncwarp();
+            ++use;
             for (int i = 0; i < t.tiles && ok; ++i, ++gt) {
-                const int s = gt & 1;
+                if ((gt & 1) != s) continue;
                 if (gt >= 2 && !(ok = mbar_wait_fast(sfree + s, (uint32_t)((gt >> 1) - 1) & 1u, 75))) break;
-                const uint32_t d = tmem + TP_TM_S + (uint32_t)(s * TA_TILE);
 #pragma unroll
                 for (int j = 0; j < 3; ++j) {
-                    if (!(ok = mbar_wait_fast(ufull + u, (uint32_t)uph, 76))) break;
+                    if (!(ok = mbar_wait_fast(full + j, (uint32_t)use & 1u, 76))) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint64_t k0 = desc_sw128(base + u * L::UNIT, 16, 1024);
 #pragma unroll
                         for (int c = 0; c < 3; ++c)
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk)
-                                mma_bf16_ts(d, tmem + (uint32_t)((3 * j + c) * 32 + kk * 8), k0 + ((c * L::CHUNK + kk * 32) >> 4), L::IDESC_QK,
-                                            (j | c | kk) != 0 ? 1u : 0u);
-                        mma_commit(ufree + u);
+                                mma_bf16_ts(d, tmem + (uint32_t)((3 * j + c) * 32 + kk * 8), k0 + (((3 * j + c) * L::CHUNK + kk * 32) >> 4),
+                                            L::IDESC_QK, (j | c | kk) != 0 ? 1u : 0u);
+                        mma_commit(free_ + j);
                         if (j == 2) mma_commit(sfull + s);
                     }
                     __syncwarp();
-                    advance();
                 }
-            }
-        }
-    } else if (score && warp == 6) {
-        // ---------------- score CTA: P to the value CTA ----------------
-        int gt = 0;
-        for (int k = 0; ok; ++k) {
-            TpItem t;
-            if (!(ok = take(k, t)) || t.rows == 0) break;
-            for (int i = 0; i < t.tiles; ++i, ++gt) {
-                const int b = gt & 1;
-                if (!(ok = mbar_wait_fast(pstaged + b, (uint32_t)(gt >> 1) & 1u, 77))) break;
-                if (elect_one()) {  // its space there is free: the rows waited for that before they wrote
-                    const uint32_t bar = dsmem_addr(pfull + b, 1);
-                    bulk_s2s(dsmem_addr(smem + L::OFF_P + b * L::P, 1), base + L::OFF_PS + b * L::P, L::P, bar);
-                    bulk_s2s(dsmem_addr(alpha_sh + 128 * b, 1), smem_u32(alpha_sh + 128 * b), 512, bar);
-                }
-                __syncwarp();
+                ++use;
             }
         }
     } else if (score) {
-        // ---------------- score CTA: softmax, one row a thread (warps 0-3) ----------------
-        const int r = tid, half = r >> 6;
-        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
-        int u = 0, uph = 0, gt = 0;  // ring position of the item's first unit
+        // ---------------- score CTA: softmax of even (warps 0-3) or odd tiles (4-7), one row a thread ----------------
+        const int r = tid & 127, half = r >> 6, s = tid >> 7, quarter = warp & 3;
+        const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+        int gt = 0, tiles_of[2] = {0, 0};  // the CTA's tiles so far, even and odd
+        // scores are scaled inside the exponent's multiply-add, so maxima are of raw scores: a negative scale
+        // flips them once, and none at all (every key alike) is as good as a tiny one
+        const bool flip = p.scale_log2 < 0.f;
+        const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
+        const uint32_t p_here = base + L::OFF_PS + (uint32_t)r * 128u;
         for (int k = 0; ok; ++k) {
             TpItem t;
             if (!(ok = take(k, t)) || t.rows == 0) break;
-            // this row's query into tensor memory (every QK of the item before is done: its scores were read)
-            int qu = u, qph = uph;
-            for (int j = 0; j < 3 * half; ++j)
-                if (++qu == TP_UNITS) {
-                    qu = 0;
-                    qph ^= 1;
-                }
-            for (int j = 0; j < 3 && ok; ++j) {
-                if (!(ok = mbar_wait_fast(ufull + qu, (uint32_t)qph, 78))) break;
-                const uint32_t src = base + qu * L::UNIT + (uint32_t)(r & 63) * 128u;
+            // this row's query into tensor memory, two thirds by warps 0-3, one by 4-7 (every QK of the item
+            // before is done: its last scores were read)
+            const uint32_t qph = (uint32_t)(k + tiles_of[half]) & 1u;  // the space of the node's query was filled that often
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+                if ((j == 2) != (s == 1)) continue;
+                if (!(ok = mbar_wait_fast(ufull + 3 * half + j, qph, 78))) break;
+                const uint32_t src = base + (uint32_t)(3 * half + j) * L::UNIT + (uint32_t)(r & 63) * 128u;
 #pragma unroll
                 for (int c = 0; c < 3; ++c) {
                     uint32_t v[32];
@@ -373,24 +382,18 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                     }
                     tmem_st32(tmem + lanes + (uint32_t)((3 * j + c) * 32), v);
                 }
-                if (++qu == TP_UNITS) {
-                    qu = 0;
-                    qph ^= 1;
-                }
             }
             if (!ok) break;
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(qtmem);
-            {  // on to the next item's first unit
-                const int n = u + 6 + 3 * t.tiles;
-                uph ^= (n / TP_UNITS) & 1;
-                u = n % TP_UNITS;
-            }
+            tiles_of[gt & 1] += (t.tiles + 1) / 2;
+            tiles_of[(gt & 1) ^ 1] += t.tiles / 2;
             const unsigned long long see = t.see[half];
-            float m_run = -INFINITY, l_run = 0.f;
+            float m_mine = -INFINITY, l_run = 0.f;  // this half's sum, and the maximum that it is relative to
             for (int i = 0; i < t.tiles; ++i, ++gt) {
-                const int s = gt & 1;
+                if ((gt & 1) != s) continue;
+                const int pb = gt & 3;
                 if (!(ok = mbar_wait_fast(sfull + s, (uint32_t)(gt >> 1) & 1u, 79))) break;
                 tc_fence_after();
                 float sv[64];
@@ -398,34 +401,36 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                 tc_fence_before();
                 mbar_arrive(sfree + s);
                 const unsigned long long bits = tree_tile_mask(see, t.pos0 + i * TA_TILE, t.ctx) & ~lost_sh[gt & 7];
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (bits == ~0ull) {
+                if (flip) {
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) {
-                        sv[j] *= p.scale_log2;
-                        top[j & 3] = fmaxf(top[j & 3], sv[j]);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 64; ++j) {
-                        sv[j] = (bits >> j) & 1 ? sv[j] * p.scale_log2 : -INFINITY;
-                        top[j & 3] = fmaxf(top[j & 3], sv[j]);
-                    }
+                    for (int j = 0; j < 64; ++j) sv[j] = -sv[j];
                 }
-                const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                if (bits != ~0ull) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) sv[j] = (bits >> j) & 1 ? sv[j] : -INFINITY;
+                }
+                float top[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+                for (int j = 4; j < 64; ++j) top[j & 3] = fmaxf(top[j & 3], sv[j]);
+                const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+                // the row's maximum runs through all tiles: from the other half's tile before to its next
+                if (gt > 0 && !(ok = mbar_wait_fast(mready + (s ^ 1), (uint32_t)((gt - 1) >> 1) & 1u, 90))) break;
+                const float m_run = i == 0 ? -INFINITY : max_sh[128 * (s ^ 1) + r];
                 const float m_new = (m_run == -INFINITY || tmax > m_run + PF_RESCALE_LOG2) ? tmax : m_run;
+                max_sh[128 * s + r] = m_new;
+                mbar_arrive(mready + s);
                 const float m_use = m_new == -INFINITY ? 0.f : m_new;
                 const float alpha = m_run == -INFINITY ? 0.f : exp2_ftz(m_run - m_new);
-                // P's place here and there: the P.V of two tiles before has read it
-                if (gt >= 2 && !(ok = mbar_wait_cluster(pfree + s, (uint32_t)((gt >> 1) - 1) & 1u, 80))) break;
-                const uint32_t prow = base + L::OFF_PS + s * L::P + (uint32_t)r * 128u;
+                // P's place, here and there: the P.V of four tiles before has read it
+                if (gt >= 4 && !(ok = mbar_wait_cluster(pfree + pb, (uint32_t)((gt >> 2) - 1) & 1u, 80))) break;
+                const uint32_t prow = p_here + (uint32_t)pb * L::P;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     uint32_t w[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const float e0 = exp2_ftz(sv[8 * c + 2 * x] - m_use), e1 = exp2_ftz(sv[8 * c + 2 * x + 1] - m_use);
+                        const float e0 = exp2_ftz(fmaf(sv[8 * c + 2 * x], scale, -m_use)), e1 = exp2_ftz(fmaf(sv[8 * c + 2 * x + 1], scale, -m_use));
                         const __nv_bfloat162 b2 = __floats2bfloat162_rn(e0, e1);
                         w[x] = *reinterpret_cast<const uint32_t*>(&b2);
                         sum[x] += e0 + e1;
@@ -433,16 +438,32 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                     sts_v4(prow + (uint32_t)((c ^ r) & 7) * 16u, make_uint4(w[0], w[1], w[2], w[3]));
                 }
                 // O moves to the new maximum only after the item's first tile
-                alpha_sh[128 * s + r] = i == 0 || m_new == m_run ? 1.f : alpha;
-                l_run = l_run * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-                m_run = m_new;
-                fence_proxy_async_smem();  // P and the factors leave by an async copy
-                mbar_arrive(pstaged + s);
+                alpha_sh[128 * pb + r] = i == 0 || m_new == m_run ? 1.f : alpha;
+                l_run = l_run * (m_mine == -INFINITY ? 0.f : exp2_ftz(m_mine - m_new)) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                m_mine = m_new;
+                fence_proxy_async_smem();  // the copies read this warp's writes
+                __syncwarp();
+                if (elect_one()) {
+                    const uint32_t bar = dsmem_addr(pfull + pb, 1), row0 = 32u * quarter;
+                    bulk_s2s(dsmem_addr(smem + L::OFF_P + pb * L::P + row0 * 128u, 1), base + L::OFF_PS + pb * L::P + row0 * 128u, 4096, bar);
+                    bulk_s2s(dsmem_addr(alpha_sh + 128 * pb + row0, 1), smem_u32(alpha_sh + 128 * pb + row0), 128, bar);
+                }
+                __syncwarp();
             }
             if (!ok) break;
+            // the half without the item's last tile hands its sum to the other
+            if (((gt - 1) & 1) != s) {
+                sum_sh[r] = make_float2(l_run, m_mine);
+                mbar_arrive(lready);
+                if (!(ok = mbar_wait_fast(ldone, (uint32_t)k & 1u, 91))) break;
+                continue;  // every QK of the item is done
+            }
+            if (!(ok = mbar_wait_fast(lready, (uint32_t)k & 1u, 92))) break;
+            const float2 other = sum_sh[r];
+            l_run += other.x * (other.y == -INFINITY ? 1.f : exp2_ftz(other.y - m_mine));  // (its sum is then 0, or NaN)
             const bool any = l_run != 0.f;  // (NaN counts: it reaches the result)
             if (half < t.rows) {
-                const float lse = any ? (m_run + log2f(l_run)) * 0.69314718055994531f : -INFINITY;
+                const float lse = any ? (m_mine + log2f(l_run)) * 0.69314718055994531f : -INFINITY;
                 const int h = r & 63;
                 if (t.part >= 0) p.lse_part[(long long)(t.part + half * t.runs) * AT_H + h] = lse;
                 else if (p.lse) p.lse[(long long)(t.row0 + half) * AT_H + h] = lse;
@@ -450,73 +471,65 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
             if (k >= 1 && !(ok = mbar_wait_cluster(finfree, (uint32_t)(k - 1) & 1u, 81))) break;
             dsmem_st_f32(dsmem_addr(fin_sh + r, 1), any ? 1.f / l_run : 0.f);
             mbar_arrive_remote(dsmem_addr(finfull, 1));
+            mbar_arrive(ldone);
+            if (!(ok = mbar_wait_fast(ldone, (uint32_t)k & 1u, 91))) break;  // all of its threads are this far
         }
-    } else if (warp == 5) {
+    } else if (warp == TP_MMA_WARP) {
         // ---------------- value CTA: P V ----------------
-        int v = 0, vph = 0, gt = 0;
-        for (int k = 0; ok; ++k) {
-            TpItem t;
-            if (!(ok = take(k, t)) || t.rows == 0) break;
-            for (int i = 0; i < t.tiles && ok; ++i, ++gt) {
-                const int b = gt & 1;
-                if (!(ok = mbar_wait_fast(pok, (uint32_t)gt & 1u, 82) && mbar_wait_fast(pfull + b, (uint32_t)(gt >> 1) & 1u, 82))) break;
-                const uint64_t p0 = desc_sw128(base + L::OFF_P + b * L::P, 16, 1024);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (!(ok = mbar_wait_fast(vfull + 2 * v + half, (uint32_t)vph, 83))) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t v0 = desc_sw128(base + v * L::VTILE + half * L::HALF, L::CHUNK, 1024);
-#pragma unroll
-                        for (int ks = 0; ks < TA_TILE / 16; ++ks)
-                            mma_bf16(tmem + (uint32_t)(half * 256), p0 + ks * 2, v0 + ((ks * 2048) >> 4), L::IDESC_PV, (i > 0 || ks > 0) ? 1u : 0u);
-                        if (i + 1 < t.tiles) mma_commit(vfree + 2 * v + half);  // the item's last: its output goes through this space
-                        if (half == 1) mma_commit(pvdone + b);
-                    }
-                    __syncwarp();
-                }
-                if (++v == TP_VBUF) {
-                    v = 0;
-                    vph ^= 1;
-                }
-            }
-        }
-    } else if (warp == 6) {
-        // ---------------- value CTA: P's space is free again ----------------
         int gt = 0;
         for (int k = 0; ok; ++k) {
             TpItem t;
             if (!(ok = take(k, t)) || t.rows == 0) break;
-            for (int i = 0; i < t.tiles; ++i, ++gt) {
-                if (!(ok = mbar_wait_fast(pvdone + (gt & 1), (uint32_t)(gt >> 1) & 1u, 84))) break;
-                if (elect_one()) mbar_arrive_remote(dsmem_addr(pfree + (gt & 1), 0));
-                __syncwarp();
+            for (int i = 0; i < t.tiles && ok; ++i, ++gt) {
+                const int pb = gt & 3, v = 2 * (gt & 1);
+                if (!(ok = mbar_wait_fast(pok + pb, (uint32_t)(gt >> 2) & 1u, 82))) break;  // P is here, O at its maximum
+                const uint64_t p0 = desc_sw128(base + L::OFF_P + pb * L::P, 16, 1024);
+                const uint64_t v0 = desc_sw128(base + v * L::HALF, L::CHUNK, 1024);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (!(ok = mbar_wait_fast(vfull + v + half, (uint32_t)(gt >> 1) & 1u, 83))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 0; ks < TA_TILE / 16; ++ks)
+                            mma_bf16(tmem + (uint32_t)(half * 256), p0 + ks * 2, v0 + ((half * L::HALF + ks * 2048) >> 4), L::IDESC_PV,
+                                     (i > 0 || ks > 0) ? 1u : 0u);
+                        if (i + 1 < t.tiles) mma_commit(vfree + v + half);  // the item's last tile: its output goes through this space
+                        if (half == 1) {
+                            mma_commit(pvdone + pb);
+                            mma_commit_cluster(pfree + pb, 1);  // P's place is free, to the score CTA
+                        }
+                    }
+                    __syncwarp();
+                }
             }
         }
-    } else {
+    } else if (warp < 4) {
         // ---------------- value CTA: rescale and output, one row a thread (warps 0-3) ----------------
         const int r = tid, half = r >> 6;
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
-        int v = 0, vph = 0, gt = 0;
+        int gt = 0;
+        auto pv_done = [&](int tile, unsigned site) -> bool { return mbar_wait_fast(pvdone + (tile & 3), (uint32_t)(tile >> 2) & 1u, site); };
         for (int k = 0; ok; ++k) {
             TpItem t;
             if (!(ok = take(k, t)) || t.rows == 0) break;
-            int last_v = 0;
             for (int i = 0; i < t.tiles; ++i, ++gt) {
-                const int b = gt & 1, pos = t.pos0 + i * TA_TILE;
-                if (!(ok = mbar_wait_fast(pfull + b, (uint32_t)(gt >> 1) & 1u, 85))) break;
-                if (tid == 0) mbar_expect_tx(pfull + b, L::COPY);  // for the P of two tiles on
-                const float alpha = alpha_sh[128 * b + r];
+                const int pos = t.pos0 + i * TA_TILE;
+                const int pb = gt & 3, v = 2 * (gt & 1);
+                if (!(ok = mbar_wait_fast(pfull + pb, (uint32_t)(gt >> 2) & 1u, 85))) break;
+                if (tid == 0) mbar_expect_tx(pfull + pb, L::P + 512);  // for the P of four tiles on
+                const float alpha = alpha_sh[128 * pb + r];
+                // (the loader's word on the tile is read once its keys are here)
+                if (!(ok = mbar_wait_fast(vfull + v, (uint32_t)(gt >> 1) & 1u, 86) && mbar_wait_fast(vfull + v + 1, (uint32_t)(gt >> 1) & 1u, 86))) break;
                 const unsigned long long lost = lost_sh[gt & 7];
                 if (pos + TA_TILE > t.ctx || lost != 0) {  // rows that not both nodes see
-                    if (!(ok = mbar_wait_fast(vfull + 2 * v, (uint32_t)vph, 86) && mbar_wait_fast(vfull + 2 * v + 1, (uint32_t)vph, 86))) break;
                     const unsigned long long m0 = tree_tile_mask(t.see[0], pos, t.ctx) & ~lost, m1 = tree_tile_mask(t.see[1], pos, t.ctx) & ~lost;
                     for (int j = warp; j < TA_TILE; j += 4) {
                         if (((m0 & m1) >> j) & 1) continue;
                         const bool one = ((m0 | m1) >> j) & 1;
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const uint32_t at = base + v * L::VTILE + (uint32_t)((lane >> 3) + 4 * x) * L::CHUNK + (uint32_t)j * 128u + (uint32_t)(lane & 7) * 16u;
+                            const uint32_t at = base + (uint32_t)(v + x) * L::HALF + (uint32_t)(lane >> 3) * L::CHUNK + (uint32_t)j * 128u + (uint32_t)(lane & 7) * 16u;
                             uint4 w = make_uint4(0, 0, 0, 0);
                             if (one) {
                                 w = lds_v4(at);
@@ -525,10 +538,9 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                             sts_v4(at, w);
                         }
                     }
-                    fence_proxy_async_smem();
                 }
-                if (__any_sync(0xffffffffu, alpha != 1.f)) {
-                    if (gt >= 1 && !(ok = mbar_wait_fast(pvdone + (b ^ 1), (uint32_t)((gt - 1) >> 1) & 1u, 87))) break;
+                if (__any_sync(0xffffffffu, alpha != 1.f)) {  // never at an item's first tile
+                    if (!(ok = pv_done(gt - 1, 87))) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < AT_DV; c += 32) {
@@ -540,16 +552,12 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                     }
                     tmem_wait_st();
                 }
+                fence_proxy_async_smem();  // cleared rows are read by the tensor cores
                 tc_fence_before();
-                mbar_arrive(pok);
-                last_v = v;
-                if (++v == TP_VBUF) {
-                    v = 0;
-                    vph ^= 1;
-                }
+                mbar_arrive(pok + pb);
             }
             if (!ok) break;
-            if (!(ok = mbar_wait_fast(pvdone + ((gt - 1) & 1), (uint32_t)((gt - 1) >> 1) & 1u, 88) && mbar_wait_cluster(finfull, (uint32_t)k & 1u, 89))) break;
+            if (!(ok = pv_done(gt - 1, 88) && mbar_wait_cluster(finfull, (uint32_t)k & 1u, 89))) break;
             tc_fence_after();
             const float inv = fin_sh[r];
             __syncwarp();
@@ -557,7 +565,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
             // O / l through the last tile's space, 128-byte pieces of this warp's 32 rows in four boxes of 4 KB
             const bool narrow = t.part < 0 && p.ctx_bf16, there = half < t.rows;
             const int y = (t.part >= 0 ? t.part + half * t.runs : t.row0 + half) * AT_H + 32 * (warp & 1);
-            const uint32_t space = base + last_v * L::VTILE + warp * 16384u, mine = space + (uint32_t)lane * 128u;
+            const int v = 2 * ((gt - 1) & 1);
+            const uint32_t space = base + (uint32_t)v * L::HALF + warp * 16384u, mine = space + (uint32_t)lane * 128u;
             auto piece = [&](int box, int seg, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
                 sts_v4(mine + (uint32_t)box * 4096u + (uint32_t)((seg ^ lane) & 7) * 16u, make_uint4(a, b, c, d));
             };
@@ -610,8 +619,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                 __threadfence_block();
                 if (atomicAdd(out_done, 1) == 3) {  // the last of the four warps gives the space back
                     *out_done = 0;
-                    mbar_arrive(vfree + 2 * last_v);
-                    mbar_arrive(vfree + 2 * last_v + 1);
+                    mbar_arrive(vfree + v);
+                    mbar_arrive(vfree + v + 1);
                 }
             }
             __syncwarp();
@@ -625,7 +634,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();  // the other CTA may still arrive on this one's barriers
-    if (warp == 5) {
+    if (warp == TP_MMA_WARP) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
