@@ -229,6 +229,8 @@ CASES = [
     ([128], [64], 64), ([0], [64], 8), ([1000], [1], 64), ([515], [9], 48), ([777], [33], 256), ([90], [5], 24),
     ([0, 65, 3, 700], [3, 0, 17, 1], 16), ([40, 0, 0, 129], [0, 0, 5, 2], 8), ([3000], [4], 32),
     ([5, 260, 1031, 64, 0, 2, 77], [1, 2, 3, 4, 5, 6, 7], 40),
+    # trees of many nodes: odd ones, requests without any, tiles that are all drafts
+    ([0, 65, 3, 700], [13, 0, 27, 1], 16), ([63, 0], [12, 0], 64), ([0], [63], 8), ([1, 129, 4100], [17, 16, 15], 48),
 ]
 
 
@@ -246,9 +248,35 @@ def test_row_strides(row, split):
 
 
 @pytest.mark.parametrize("spread", [0.01, 6.0])
-def test_flat_and_peaked_scores(spread):
-    t = Trees([900, 3], [6, 1], 16, seed=5, spread=spread)
+@pytest.mark.parametrize("nodes", [[6, 1], [21, 4]])
+def test_flat_and_peaked_scores(spread, nodes):
+    t = Trees([900, 3], nodes, 16, seed=5, spread=spread)
     t.check(t.call())
+
+
+@pytest.mark.parametrize("nodes", [[2], [13]])
+def test_the_maximum_that_grows_tile_by_tile(nodes):
+    """Keys of growing size, so that O is rescaled again and again, in every split."""
+    t = Trees([1500], nodes, 64, seed=23)
+    pos = np.arange(1500 + nodes[0])
+    slots = torch.from_numpy(t.table[0][pos // 64].astype(np.int64) * 64 + pos % 64).cuda()
+    grow = torch.linspace(0.05, 6, len(pos), device="cuda")[:, None]
+    for pool in (t.c_kv, t.k_rot):
+        pool[slots] = (pool[slots].float() * grow).to(torch.bfloat16)
+    t.check(t.call())
+
+
+@pytest.mark.parametrize("scale", [-0.0625, 0.0, 0.3])
+@pytest.mark.parametrize("nodes", [[2], [13]])
+def test_other_softmax_scales(scale, nodes):
+    t = Trees([300], nodes, 16, seed=24, spread=0.3)
+    cfg = A.glm52_cfg(T_MAX)
+    cfg.softmax_scale = scale
+    got = P.mla_tree_attn(cfg, t.kv(), t.q, i32(t.ctx), i32(t.cu), parent=i32(t.parent))
+    q, rows = t.q.float().cpu().numpy(), t.rows()
+    ref, lse, a = R.tree_attn(q, rows, t.ctx, t.cu, t.masks, t.table, t.page, scale)
+    assert np.all(np.abs(cpu(got["ctx"]) - ref) <= (2.0 ** -8 + 1e-3) * a)
+    assert np.abs(cpu(got["lse"]) - lse).max() < 1e-3
 
 
 def test_many_requests_and_long_contexts():
@@ -284,6 +312,20 @@ def test_all_64_bits_of_a_mask():
     masks = [(1 << 64) - 1 - (1 << (j * 7 % 64)) for j in range(64)]
     signed = [m - (1 << 64) if m >= 1 << 63 else m for m in masks]
     t.check(t.call(parent=None, mask=torch.tensor(signed, dtype=torch.int64, device="cuda")), masks=masks)
+
+
+@pytest.mark.parametrize("nodes", [[13, 64], [64, 1]])
+def test_masks_of_many_nodes(nodes):
+    t = Trees([0, 70], nodes, 16, seed=21)
+    rng = np.random.default_rng(21)
+    masks = [int(rng.integers(0, 1 << 62)) & int(rng.integers(0, 1 << 62)) | int(rng.integers(0, 4)) << 62 for _ in range(t.n)]
+    masks[0] = masks[3] = 0  # request 0 has no context: these rows see nothing
+    masks = [m & ((1 << nodes[0 if r < nodes[0] else 1]) - 1) for r, m in enumerate(masks)]
+    junk = [m | (1 << 40 if n < 40 else 0) for m, n in zip(masks, [nodes[0]] * nodes[0] + [nodes[1]] * nodes[1])]  # bits of no node
+    signed = [m - (1 << 64) if m >= 1 << 63 else m for m in junk]
+    got = t.call(parent=None, mask=torch.tensor(signed, dtype=torch.int64, device="cuda"))
+    t.check(got, masks=masks)
+    assert (cpu(got["ctx"])[[0, 3]] == 0).all() and np.isneginf(cpu(got["lse"])[[0, 3]]).all()
 
 
 def test_chain_is_the_default():
@@ -327,12 +369,44 @@ def test_unseen_rows_never_reach_a_result(junk, with_sel):
     t.c_kv[slot], t.k_rot[slot] = clean
 
 
-def test_rows_behind_the_last_request_stay():
-    t = Trees([50, 20], [3, 2], 16, seed=10, spare_rows=4)
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf"), torch.finfo(torch.bfloat16).min])
+def test_unseen_rows_of_many_nodes(junk):
+    """As above for trees whose nodes are worked on two at a time: a junk row may be seen by one of the two."""
+    ctx, nodes = [70, 5], [15, 10]
+    t = Trees(ctx, nodes, 16, seed=22)
+    used = np.zeros(t.n_pages * 16, bool)
+    for b in range(2):
+        p = np.arange(ctx[b] + nodes[b])
+        used[t.table[b][p // 16] * 16 + p % 16] = True
+    gone = torch.from_numpy(np.flatnonzero(~used)).cuda()
+    for pool in (t.c_kv, t.k_rot):
+        pool[gone] = junk
+    masks = [1 << (r if r < 15 else r - 15) for r in range(25)]  # each node itself
+    seers = {4: [4, 7, 8, 9], 11: [2, 11]}  # junk drafts of request 0, and who sees them: one or both of a pair
+    for j, rows in seers.items():
+        for r in rows:
+            masks[r] |= 1 << j
+    kw = dict(parent=None, mask=torch.tensor(masks, dtype=torch.int64, device="cuda"))
+    want = t.call(**kw)
+    t.check(want, masks=masks)
+    for j in seers:
+        slot = int(t.table[0][(70 + j) // 16] * 16 + (70 + j) % 16)
+        t.c_kv[slot], t.k_rot[slot] = junk, junk
+    got = t.call(**kw)
+    same = [r for r in range(25) if not any(r in rows for rows in seers.values())]
+    assert torch.equal(got["ctx"][same], want["ctx"][same]) and torch.equal(got["lse"][same], want["lse"][same])
+    if junk != junk:
+        seen = sorted(set(sum(seers.values(), [])))
+        assert torch.isnan(got["ctx"][seen]).all() and torch.isnan(got["lse"][seen]).all()
+
+
+@pytest.mark.parametrize("nodes", [[3, 2], [20, 9]])
+def test_rows_behind_the_last_request_stay(nodes):
+    t = Trees([50, 20], nodes, 16, seed=10, spare_rows=4)
     ctx = torch.full((t.n, 64, 512), 7.0, device="cuda")
     lse = torch.full((t.n, 64), 9.0, device="cuda")
     t.check(t.call(ctx=ctx, lse=lse))
-    assert (ctx[5:] == 7).all() and (lse[5:] == 9).all()
+    assert (ctx[sum(nodes):] == 7).all() and (lse[sum(nodes):] == 9).all()
 
 
 SEL_CASES = [([300], [4], 16, 64), ([300], [4], 16, 65), ([2000, 40, 0], [3, 0, 9], 64, 256), ([5], [2], 8, 1),
@@ -409,17 +483,19 @@ def test_bad_numbers_are_flagged_and_skipped():
     assert (ctx == 7).all()
 
 
-def test_a_page_outside_the_pool_is_flagged_and_left_out():
-    t = Trees([100], [2], 16, seed=16)
-    keep = np.r_[np.arange(32), np.arange(48, 102)]  # page 2 of the request is bad
-    t.table[0, 2] = t.n_pages
+@pytest.mark.parametrize("n", [2, 14])
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+def test_a_page_outside_the_pool_is_flagged_and_left_out(n, bad):
+    t = Trees([100], [n], 16, seed=16)
+    keep = np.r_[np.arange(32), np.arange(48, 100 + n)]  # page 2 of the request is bad
+    t.table[0, 2] = bad
     got = t.call()
     bad_word()
-    sel = t.call(sel_in=i32(np.tile(np.arange(102), (2, 1))))
+    sel = t.call(sel_in=i32(np.tile(np.arange(100 + n), (n, 1))))
     bad_word()
     t.table[0, 2] = 0
-    t.check(got, sel=[keep, keep])
-    t.check(sel, sel=[keep, keep])
+    t.check(got, sel=[keep] * n)
+    t.check(sel, sel=[keep] * n)
 
 
 def test_graph_replays_follow_the_lengths_and_streams_do_not_mix():

@@ -123,7 +123,7 @@ constexpr int TA_NBUF = 3;
 constexpr int TA_LOAD_WARP = 4;       // warps 0-3 softmax, then the loaders (dense 1 warp, lists 8), then MMA
 constexpr int TA_SCHED_THREADS = 192;
 constexpr int TA_MAX_BATCH = 16384;   // the schedule's table of a CTA (8 bytes a request) fits the key tiles' space
-constexpr int TA_CANDS = 64;          // candidate splits: 1..32, then 36, 40, .. 160 (3 x TA_CANDS threads sum up)
+constexpr int TA_CANDS = 64;          // candidate splits: 1, 1.25, .. 8.75, 9 .. 24, then 32.5, 41, .. 160 (3 x TA_CANDS threads sum up)
 constexpr int TA_MAX_SPLIT = 160;
 // Costs in key tiles of one CTA (1.25 us): an item's query, output and pipeline fill; a partial written and
 // joined, and one beyond a round of the CTAs. Fitted on 16 workloads of 1 to 230 nodes: the second price keeps
@@ -191,14 +191,19 @@ struct TreeCost {
     int items[3][TA_CANDS], parts[3][TA_CANDS];
     float sum[3][TA_CANDS], last[3][TA_CANDS];
 };
-__device__ __forceinline__ int tree_candidate(int c) { return c < 32 ? c + 1 : 32 + 4 * (c - 31); }
+// Runs of the longest request, and from them the tiles a run has at most. (Fractions: requests of other lengths
+// then find a C between the whole parts of the longest; 32 requests of 4-8K: 130 runs of 26 tiles become 142 of 23.)
+__device__ __forceinline__ float tree_candidate(int c) {
+    return c < 32 ? 1.f + 0.25f * c : c < 48 ? 9.f + (c - 32) : 24.f + 8.5f * (c - 47);
+}
+__device__ __forceinline__ int tree_run_tiles(int longest, float s) { return max(1, (int)ceilf(__fdividef((float)longest, s))); }
 
 template <int PER>  // nodes an item takes
 __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* tab, int longest, TreeCost* acc, int G, TreePrice price,
                                              int last_warp = TA_LOAD_WARP) {
     const int cand = threadIdx.x % TA_CANDS, grp = threadIdx.x / TA_CANDS;
     const int per = (p.batch + 2) / 3, b0 = min(grp * per, p.batch), b1 = min(b0 + per, p.batch);
-    const int s = tree_candidate(cand), C = max(1, div_near(longest + s - 1, s, __fdividef(1.f, (float)s)));
+    const int C = tree_run_tiles(longest, tree_candidate(cand));
     const float inv = __fdividef(1.f, (float)C);
     const bool mine = threadIdx.x < TA_SCHED_THREADS;
     if (mine) {
@@ -234,8 +239,7 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
     __syncthreads();
     if ((int)threadIdx.x / 32 != last_warp) return 0;
     const int lane = threadIdx.x & 31;
-    float best = 3e38f;
-    int best_s = 1;
+    float best = 3e38f, best_s = 1.f;
     const float inv_g = __fdividef(1.f, (float)G);
 #pragma unroll
     for (int c = lane; c < TA_CANDS; c += 32) {
@@ -251,13 +255,13 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
 #pragma unroll 1
     for (int o = 16; o > 0; o >>= 1) {
         const float c = __shfl_xor_sync(0xffffffffu, best, o);
-        const int t = __shfl_xor_sync(0xffffffffu, best_s, o);
+        const float t = __shfl_xor_sync(0xffffffffu, best_s, o);
         if (c < best || (c == best && t < best_s)) {
             best = c;
             best_s = t;
         }
     }
-    return max(1, div_near(longest + best_s - 1, best_s, __fdividef(1.f, (float)best_s)));
+    return tree_run_tiles(longest, best_s);
 }
 // Worker me's item of round k: the G workers take them forth and back.
 __device__ __forceinline__ int item_of(int k, int me, int G) { return k * G + ((k & 1) ? G - 1 - me : me); }

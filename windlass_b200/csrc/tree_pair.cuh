@@ -39,7 +39,7 @@ constexpr int TP_UNITS = 6;   // score CTA: [even, odd][3] thirds of a tile (64 
 constexpr int TP_HALVES = 4;  // value CTA: [even, odd][2] halves of a tile (64 keys x 256 columns)
 constexpr int TP_P = 4;       // value CTA: tiles of P (score CTA: on their way), tile & 3
 constexpr uint32_t TP_TM_S = 384;  // score columns in tensor memory (the queries take [0, 288))
-constexpr TreePrice TP_PRICE = {9.f, 0.08f, 0.16f};
+constexpr TreePrice TP_PRICE = {6.f, 0.12f, 0.2f};  // (0.8 us a tile; see TA_PRICE)
 
 struct TpLayout {
     static constexpr uint32_t CHUNK = TA_TILE * 128;          // 8 KB: 64 keys x 64 columns

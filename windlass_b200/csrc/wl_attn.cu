@@ -1435,9 +1435,11 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     p.box_rows = (kv.page_size & -kv.page_size) < wl::TA_TILE ? (kv.page_size & -kv.page_size) : wl::TA_TILE;
     wl::TreeMaps tm{};
     if (int e = encode_q_map(&tm.q, io->q_abs, io->n_nodes)) return e;
-    // Two nodes of a request at a time, by CTA pairs, when requests have two and more on average; one at a time
-    // otherwise (a lone node leaves half of a pair's rows empty), and for lists (a list per node).
-    const bool pairs = !p.sel && 2 * (int64_t)io->n_nodes >= 3 * (int64_t)io->batch;
+    // Two nodes of a request at a time, by CTA pairs, for trees of six and more nodes; one at a time for smaller
+    // ones (a lone or last odd node leaves half of a pair's rows empty, and with little work the pair's longer
+    // start and end show) and for lists (a list per node). One at a time / pairs, us: 20 nodes of 4 requests, 4K
+    // keys 31 / 35; 40 of 17, 13K 94 / 99; 90 of 15, 2.6K 65 / 54; 92 of 8, 16K 208 / 191; 394 of 16, 32K 1600 / 1318.
+    const bool pairs = !p.sel && io->n_nodes >= 12 && (int64_t)io->n_nodes >= 6 * (int64_t)io->batch;
     const uint32_t out_rows = pairs ? 32 : 16;  // a warp's rows
     if (int e = encode_out_map(&tm.part, p.o_part, parts, false, out_rows)) return e;
     if (int e = encode_out_map(&tm.out, io->ctx, io->n_nodes, p.ctx_bf16, out_rows)) return e;
