@@ -20,8 +20,9 @@
 //   loaders   the item's query (one ring entry), then its key tiles. Dense: one
 //             warp issues TMA boxes, one per page part and 64 columns, so the
 //             128B-swizzled tile needs no threads. Lists: 8 warps gather rows with
-//             16-byte cp.async, two tiles in flight (TMA gather4 of four rows x 64
-//             columns took twice as long a tile). A tile comes and goes in two
+//             16-byte cp.async (80 bytes a cycle and SM from L2; TMA gather4 of four
+//             rows x 64 columns at best 35), each half of a tile reported by
+//             its copies' own arrival. A tile comes and goes in two
 //             halves (columns 0-255 and the roped ones; columns 256-511): QK
 //             starts on the first while the second is on its way, and P.V gives
 //             the first back while it reads the second.
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int b = 0; b < 2 * TA_NBUF; ++b) {
-            mbar_init(kfull + b, SEL ? L::LOADERS : 1);
+            mbar_init(kfull + b, !SEL ? 1 : L::LOADERS + (b & 1 ? 0 : 2));  // lists: and two for see_sh, with the first half
             mbar_init(kfree + b, 1);  // the P.V commit of that half; the MMA warp for a query
                                       // entry, the softmax warps for an item's last tile
         }
@@ -614,19 +615,8 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                 asm volatile("bar.sync 2, %0;" ::"n"(L::LOADERS) : "memory");
                 return go[x] != 0;  // rewritten two calls on, behind the barrier in between
             };
-            int pend = -1;  // ring slot whose copies are in flight, two groups (halves)
-            auto landed = [&](int half) {
-                fence_proxy_async_smem();
-                mbar_arrive(kfull + 2 * pend + half);
-            };
-            auto flush = [&]() {
-                if (pend < 0) return;
-                cp_async_wait<1>();
-                landed(0);
-                cp_async_wait<0>();
-                landed(1);
-                pend = -1;
-            };
+            // The first half's two further arrivals: the threads that write see_sh.
+            const bool marks = g == 0 || g == 32;
             const int r8 = g >> 3, seg = g & 7;  // this thread's 16 bytes of rows r8 and r8 + 32 of a tile
             for (int k = 0; ok; ++k) {
                 TreeItem t{};
@@ -649,7 +639,6 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                         info[7] = (int)(unsigned)(see >> 32);
                     }
                 }
-                flush();
                 if (!(ok = acquire(0))) break;  // also orders info[]
                 const int row = info[0], left = info[5], n_tiles = (left + TA_TILE - 1) / TA_TILE, ctx = info[2], n = info[3];
                 const unsigned long long see = (unsigned)info[6] | ((unsigned long long)(unsigned)info[7] << 32);
@@ -658,6 +647,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                 if (!(ok = acquire(1))) break;  // and info[] is read before the next item's
                 const int qb = e % TA_NBUF;
                 if (g == 0) items[qb] = make_int4(row, n_tiles, t.part, 0);
+                if (marks) mbar_arrive(kfull + 2 * qb);
                 if (row < 0) {
                     mbar_arrive(kfull + 2 * qb);
                     break;
@@ -696,7 +686,10 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                         page = page_of(pos);
                         nxt = entry((i + 2) * TA_TILE + g);
                         if (!(ok = acquire(0))) break;
-                        if (lane == 0) reinterpret_cast<volatile unsigned*>(see_sh + b)[g >> 5] = bits;
+                        if (marks) {
+                            reinterpret_cast<volatile unsigned*>(see_sh + b)[g >> 5] = bits;
+                            mbar_arrive(kfull + 2 * b);
+                        }
                     } else if (!(ok = acquire(0))) {
                         break;
                     }
@@ -712,27 +705,18 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     }
                     cp_async16(dst + 8 * L::CHUNK, p.k_rot + (long long)max(sl0, 0) * p.krot_row + seg * 8, by0);
                     cp_async16(dst + 8 * L::CHUNK + 32 * 128, p.k_rot + (long long)max(sl1, 0) * p.krot_row + seg * 8, by1);
-                    cp_async_commit();
-                    if (pend >= 0) {
-                        cp_async_wait<2>();
-                        landed(0);
-                    }
+                    cp_async_arrive(kfull + 2 * b);
                     if (!(ok = acquire(1))) break;
 #pragma unroll
                     for (int c = 4; c < 8; ++c) {
                         cp_async16(dst + c * L::CHUNK, src0 + c * 64, by0);
                         cp_async16(dst + c * L::CHUNK + 32 * 128, src1 + c * 64, by1);
                     }
-                    cp_async_commit();
-                    if (pend >= 0) {
-                        cp_async_wait<2>();
-                        landed(1);
-                    }
-                    pend = b;
+                    cp_async_arrive(kfull + 2 * b + 1);
                     ++e;
                 }
             }
-            cp_async_wait<0>();
+            cp_async_wait_all();
             if (!ok && g == 0) {  // a query in flight must land before the CTA leaves
                 for (int k = 0; k < 2 * TA_NBUF; ++k) mbar_wait_fast(kfull + k, 0, 51);
             }
@@ -753,6 +737,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                                 (c | kk) != 0 ? 1u : 0u);
             };
             if (!mbar_wait_fast(kfull + 2 * b, (uint32_t)(entry / TA_NBUF) & 1u, 52)) return false;
+            if (SEL) fence_proxy_async_smem();  // gathered rows (cp.async) -> tensor cores
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
@@ -760,6 +745,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                 chunk(8);
             }
             if (!mbar_wait_fast(kfull + 2 * b + 1, (uint32_t)(entry / TA_NBUF) & 1u, 53)) return false;
+            if (SEL) fence_proxy_async_smem();
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
