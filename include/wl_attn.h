@@ -435,7 +435,10 @@ typedef struct wl_paged_kv {
  * of the call, over all requests, is free_list[n_free - 1 - k]); a request
  * whose pages do not all fit (then neither do those of later requests that
  * need any), or that would not fit its table row, gets none: short_out[b] is the
- * number of pages it lacks (0 = served) and its slots are -1. Lengths below 0
+ * number of pages it lacks (0 = served), its slots are -1, and so are the table
+ * entries of those pages (an attention or a commit over them sets the error word
+ * and leaves them out; the caller drops the request's tokens, or frees pages and
+ * plans again). Lengths below 0
  * set the device error word; such a request gets short_out[b] = -1, no pages
  * and no tokens. Tokens are laid out request after request: token i of
  * request b is row cu_new[b] + i. Rows behind the last token (a padded batch)

@@ -14,9 +14,11 @@ def page_plan(ctx, new, held, table, free, n_free, page, n_pages, n_tokens):
         need = max(0, total - held[b])
         if total > table.shape[1]:
             short.append(need)
+            table[b, held[b]:] = -1
         elif need and asked + need > n_free:
             short.append(need)
             asked += need
+            table[b, held[b]:total] = -1
         else:
             short.append(0)
             for k in range(need):

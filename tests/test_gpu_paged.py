@@ -678,3 +678,25 @@ def test_append_skips_padding_and_flags_slots_outside_the_pool():
     P.cache_append_paged(cfg, i32([32, -2, 3]), one, zero, kv=k, kv_raw=raw, kv_norm_w=norm)
     bad_word()
     assert sorted(torch.nonzero(kv.abs().sum(1)).flatten().tolist()) == [3, 9, 31]
+
+
+def test_a_request_without_pages_neither_reads_nor_moves_others_rows():
+    """Stale table entries of a request that got no pages lead nowhere: its drafts are left out and its commit
+    moves nothing, in whatever pages the entries named before."""
+    page = 16
+    pool = torch.randn(4 * page, 576, device="cuda", dtype=torch.bfloat16)
+    was = pool.clone()
+    table, held = i32([[0, 1], [2, 1]]), i32([2, 1])  # request 1's second entry names request 0's page
+    plan = P.page_plan(i32([20, 14]), i32([4, 6]), table, held, i32([3, 3, 3, 3]), i32([0]), page, 10)
+    assert cpu(plan["short"]).tolist() == [0, 1] and cpu(table).tolist() == [[0, 1], [2, -1]]
+    assert (cpu(plan["slot"])[4:] == -1).all() and int(plan["n_free"]) == 0
+    kv = P.PagedKV.packed(pool, page, table)
+    q = torch.randn(10, 64, 576, device="cuda").to(torch.bfloat16)
+    par = i32([-1, 0, 0, 0, -1, 0, 0, 0, 0, 0])
+    out = P.mla_tree_attn(A.glm52_cfg(64), kv, q, i32([20, 14]), plan["cu"], parent=par)
+    bad_word()
+    assert torch.isfinite(out["ctx"]).all()
+    tok, tgt = i32([0, 1, 2, 3, 0, 9, 9, 9, 5, 9]), i32([7, 7, 7, 7, 5, 0, 0, 0, 0, 0])  # request 1 accepts its node 4
+    P.tree_commit(P.LayerCaches([kv]), i32([20, 14]), plan["cu"], par, tok, tgt)
+    bad_word()
+    assert torch.equal(pool, was)

@@ -112,7 +112,7 @@ def page_plan(ctx_len: torch.Tensor, n_new: torch.Tensor, block_table: torch.Ten
     (``wl_page_plan``). New pages come from the top of the stack ``free_list[:n_free]`` in
     request order and are written into ``block_table``. Returns slot, pos, seq
     [n_tokens] (rows behind the last token: -1), cu [batch + 1], short [batch] (pages a
-    request lacks; such a request gets none, and slots of -1), n_held [batch] and
+    request lacks; such a request gets none, and slots and table entries of -1), n_held [batch] and
     n_free [1] after the call: new tensors, or the given ones with ``in_place``."""
     dev = ctx_len.device
     B, T = ctx_len.numel(), int(n_tokens)
