@@ -94,7 +94,7 @@ def test_plan_matches_the_restatement(B, ctx_max, new_max, page):
     check_plan(args, page, total + 13, in_place=True)  # a padded batch
 
 
-@pytest.mark.parametrize("n_tokens", [4096, 4097, 9001])
+@pytest.mark.parametrize("n_tokens", [2048, 2049, 4096, 4097, 9001])
 def test_plan_on_both_sides_of_the_second_launch(n_tokens):
     rng = np.random.default_rng(n_tokens)
     B = 11

@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(ReleaseParam
 }
 
 // ---- the commit of an accepted path ----------------------------------------------------
-constexpr int COMMIT_LAYERS = 64;   // layers of one launch (their pointers travel as a kernel argument)
+constexpr int COMMIT_LAYERS = 80;   // layers of one launch (their pointers travel as a kernel argument of 4 KB at most)
 constexpr int COMMIT_THREADS = 96;  // one 16-byte piece of a layer's rows each: 64 c_kv, 8 k_rot, 8 key, 1 scale
 
 struct CommitLayer {
@@ -287,6 +287,7 @@ struct CommitParams {
     int n_layers;  // layers of this launch
     CommitLayer layer[COMMIT_LAYERS];
 };
+static_assert(sizeof(CommitParams) <= 4096, "kernel arguments");
 
 // grid (layers or 1, batch). Warp 0 walks the request's tree in registers (two
 // nodes a lane, one ballot a step); every thread then owns one 16-byte column

@@ -844,10 +844,6 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     if (out_part >= 0) p.lse_part[(long long)out_part * AT_H + h] = lse;
                     else if (p.lse) p.lse[(long long)out_row * AT_H + h] = lse;
                 }
-                if (!hi_half) {
-                    if (out_part >= 0) p.lse_part[(long long)out_part * AT_H + h] = lse;
-                    else if (p.lse) p.lse[(long long)out_row * AT_H + h] = lse;
-                }
                 if (out_slot >= 0) {
                     // O leaves through the space of the item's last tile (its P.V is done; the MMA warp leaves it
                     // to this role to give back), a warp's 16 heads in boxes of 128 bytes a head, by TMA stores:
@@ -1010,89 +1006,108 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
 }
 
 // Joins the partials of the nodes that were cut: ctx = sum_s e^(lse_s - L) o_s,
-// L = log sum_s e^lse_s. A block owns one (head, 128 columns) of every k-th node;
-// its four warps take the parts in turn, eight loads in flight each, and add
-// their sums in warp order.
-constexpr int TM_UNITS = AT_H * (AT_DV / 128);
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
+// L = log sum_s e^lse_s. A block owns one (head, 128 columns) of every k-th node.
+// A node of up to TM_SOLO parts is joined by one warp, four nodes at a time; a
+// longer one by the four warps together, their sums added in warp order. Bound by
+// the latency of dependent loads: a warp reads TM_DEPTH partials and their lse
+// at once, and every lane works out the weights itself, with a running maximum.
+constexpr int TM_UNITS = AT_H * (AT_DV / 128), TM_WARPS = 4, TM_DEPTH = 4, TM_SOLO = 8;
+__global__ void __launch_bounds__(TM_WARPS * 32) tree_merge_kernel(const TreeParams p) {
     pdl_wait();
     pdl_trigger();
-    __shared__ float w_sh[TA_MAX_SPLIT];
-    __shared__ float4 part_sh[3][32];
+    __shared__ float4 part_sh[TM_WARPS - 1][32];
+    __shared__ float2 stat_sh[TM_WARPS - 1];
+    constexpr float LOG2E = 1.4426950408889634f;
     const int lane = threadIdx.x & 31, wi = threadIdx.x >> 5;
     const int h = (blockIdx.x % TM_UNITS) >> 2, q = blockIdx.x & 3, step = gridDim.x / TM_UNITS;
+    int turn = 0;  // of the warps at the short nodes
     for (int r0 = blockIdx.x / TM_UNITS; r0 < p.n_nodes; r0 += 32 * step) {
         const int rl = r0 + lane * step;
         const int2 mine = rl < p.n_nodes ? p.node_tab[rl] : make_int2(0, 0);
         for (unsigned cut = __ballot_sync(0xffffffffu, mine.y > 1); cut; cut &= cut - 1) {
             const int l = __ffs(cut) - 1, r = r0 + l * step;
             const int part0 = __shfl_sync(0xffffffffu, mine.x, l), n = __shfl_sync(0xffffffffu, mine.y, l);
-            // the first round of partials is under way while the weights are worked out
-            const float* src = p.o_part + ((long long)part0 * AT_H + h) * AT_DV + q * 128 + lane * 4;
-            float4 v[8];
-            auto fetch = [&](int s0) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (s0 + 4 * k < n) v[k] = *reinterpret_cast<const float4*>(src + (long long)(s0 + 4 * k) * (AT_H * AT_DV));
-            };
-            fetch(wi);
-            float ls[TA_MAX_SPLIT / 32], M = -INFINITY, W = 0.f;
-#pragma unroll
-            for (int k = 0; k < TA_MAX_SPLIT / 32; ++k) {
-                const int s = lane + 32 * k;
-                ls[k] = s < n ? p.lse_part[(long long)(part0 + s) * AT_H + h] : -INFINITY;
-                M = fmaxf(M, ls[k]);
-            }
-            for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            const float Mu = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int k = 0; k < TA_MAX_SPLIT / 32; ++k) {
-                ls[k] = exp2f((ls[k] - Mu) * 1.4426950408889634f);
-                W += ls[k];
-            }
-            for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(0xffffffffu, W, o);
-            const float inv = W != 0.f ? 1.f / W : 0.f;
-            if (wi == 0) {
-#pragma unroll
-                for (int k = 0; k < TA_MAX_SPLIT / 32; ++k)
-                    if (lane + 32 * k < n) w_sh[lane + 32 * k] = ls[k] * inv;
-            }
-            __syncthreads();
+            const bool solo = n <= TM_SOLO;
+            if (solo && (turn++ & (TM_WARPS - 1)) != wi) continue;
+            const int by = solo ? 1 : TM_WARPS;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int s0 = wi; s0 < n; s0 += 32) {
-                if (s0 > wi) fetch(s0);
+            float M = -INFINITY, W = 0.f;
+            // (M, W, acc) times e^(M - what) and more: the sums of two sets of parts by one maximum
+            auto scale_to = [&](float m_new) {
+                const float a = exp2f((M - (m_new == -INFINITY ? 0.f : m_new)) * LOG2E);
+                M = m_new;
+                W *= a;
+                acc.x *= a;
+                acc.y *= a;
+                acc.z *= a;
+                acc.w *= a;
+            };
+#pragma unroll 1
+            for (int s0 = solo ? 0 : wi; s0 < n; s0 += TM_DEPTH * by) {
+                const long long at0 = (long long)(part0 + s0) * AT_H + h, hop = (long long)by * AT_H;
+                float4 v[TM_DEPTH];
+                float ls[TM_DEPTH], m_new = M;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    if (s0 + 4 * k >= n) continue;
-                    const float w = w_sh[s0 + 4 * k];
+                for (int k = 0; k < TM_DEPTH; ++k) {
+                    const bool is = s0 + by * k < n;
+                    ls[k] = is ? p.lse_part[at0 + k * hop] : -INFINITY;
+                    v[k] = is ? *reinterpret_cast<const float4*>(p.o_part + (at0 + k * hop) * AT_DV + q * 128 + lane * 4)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < TM_DEPTH; ++k) m_new = fmaxf(m_new, ls[k]);
+                scale_to(m_new);
+                const float m_use = m_new == -INFINITY ? 0.f : m_new;
+#pragma unroll
+                for (int k = 0; k < TM_DEPTH; ++k) {
+                    const float w = exp2f((ls[k] - m_use) * LOG2E);
+                    W += w;
                     acc.x = fmaf(w, v[k].x, acc.x);
                     acc.y = fmaf(w, v[k].y, acc.y);
                     acc.z = fmaf(w, v[k].z, acc.z);
                     acc.w = fmaf(w, v[k].w, acc.w);
                 }
             }
-            if (wi > 0) part_sh[wi - 1][lane] = acc;
-            __syncthreads();
-            if (wi == 0) {
+            if (!solo) {
+                if (wi > 0) {
+                    part_sh[wi - 1][lane] = acc;
+                    if (lane == 0) stat_sh[wi - 1] = make_float2(M, W);
+                }
+                __syncthreads();
+                if (wi == 0) {
+                    float m_new = M;
 #pragma unroll
-                for (int k = 0; k < 3; ++k) {
-                    const float4 o = part_sh[k][lane];
-                    acc.x += o.x;
-                    acc.y += o.y;
-                    acc.z += o.z;
-                    acc.w += o.w;
+                    for (int k = 0; k < TM_WARPS - 1; ++k) m_new = fmaxf(m_new, stat_sh[k].x);
+                    scale_to(m_new);
+                    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+#pragma unroll
+                    for (int k = 0; k < TM_WARPS - 1; ++k) {
+                        const float4 o = part_sh[k][lane];
+                        const float w = exp2f((stat_sh[k].x - m_use) * LOG2E);
+                        W = fmaf(w, stat_sh[k].y, W);
+                        acc.x = fmaf(w, o.x, acc.x);
+                        acc.y = fmaf(w, o.y, acc.y);
+                        acc.z = fmaf(w, o.z, acc.z);
+                        acc.w = fmaf(w, o.w, acc.w);
+                    }
                 }
-                const long long at = ((long long)r * AT_H + h) * AT_DV + q * 128 + lane * 4;
-                if (p.ctx_bf16) {
-                    const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x, acc.y), c = __floats2bfloat162_rn(acc.z, acc.w);
-                    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.ctx) + at) =
-                        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
-                } else {
-                    *reinterpret_cast<float4*>(static_cast<float*>(p.ctx) + at) = acc;
-                }
-                if (q == 0 && lane == 0 && p.lse) p.lse[(long long)r * AT_H + h] = W != 0.f ? M + logf(W) : -INFINITY;
+                __syncthreads();  // the shared arrays are reused
+                if (wi > 0) continue;
             }
-            __syncthreads();  // shared arrays are reused
+            const float inv = W != 0.f ? 1.f / W : 0.f;  // (NaN counts: it reaches the result)
+            acc.x *= inv;
+            acc.y *= inv;
+            acc.z *= inv;
+            acc.w *= inv;
+            const long long at = ((long long)r * AT_H + h) * AT_DV + q * 128 + lane * 4;
+            if (p.ctx_bf16) {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x, acc.y), c = __floats2bfloat162_rn(acc.z, acc.w);
+                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.ctx) + at) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
+            } else {
+                *reinterpret_cast<float4*>(static_cast<float*>(p.ctx) + at) = acc;
+            }
+            if (q == 0 && lane == 0 && p.lse) p.lse[(long long)r * AT_H + h] = W != 0.f ? M + logf(W) : -INFINITY;
         }
     }
 }

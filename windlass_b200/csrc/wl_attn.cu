@@ -61,7 +61,9 @@ constexpr int kMaxSplits = 32;   // split-K CTAs per decode row (the merge takes
 constexpr int kMaxDevices = 64;
 // Plans of at most this many token rows run in one launch: the plan's one CTA
 // writes the rows itself. Larger ones write them from a second, wide launch.
-constexpr int kPlanOneLaunch = 4096;
+// One launch against two, us: 128 rows 3.4 / 4.4, 1024 rows 4.0 / 5.1, 2048
+// rows 4.9 / 5.1, 4096 rows 6.0 / 5.1, 16384 rows 13.7 / 5.0.
+constexpr int kPlanOneLaunch = 2048;
 
 #define WL_CUDA_TRY(expr)                                           \
     do {                                                            \
@@ -1474,7 +1476,7 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
                                wl::TaLayout<false>::BYTES, st, p, tm));
     }
     const int per = io->n_nodes < 9 ? io->n_nodes : 9;  // 9 x 256 blocks of 4 warps: one wave
-    WL_CUDA_TRY(launch_pdl(wl::tree_merge_kernel, dim3(wl::TM_UNITS * per), dim3(128), 0, st, p));
+    WL_CUDA_TRY(launch_pdl(wl::tree_merge_kernel, dim3(wl::TM_UNITS * per), dim3(wl::TM_WARPS * 32), 0, st, p));
     return WL_OK;
 }
 
