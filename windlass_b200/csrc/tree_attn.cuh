@@ -127,13 +127,13 @@ constexpr int TA_MAX_BATCH = 16384;   // the schedule's table of a CTA (8 bytes 
 constexpr int TA_CANDS = 64;          // candidate splits: 1, 1.25, .. 8.75, 9 .. 24, then 32.5, 41, .. 160 (3 x TA_CANDS threads sum up)
 constexpr int TA_MAX_SPLIT = 160;
 // Costs in key tiles of one CTA (1.25 us): an item's query, output and pipeline fill; a partial written and
-// joined, and one beyond a round of the CTAs. Fitted on 16 workloads of 1 to 230 nodes: the second price keeps
-// 15 requests x 4-8 nodes x 2.6K keys whole (64.6 us, 78.2 in runs) and 8 x 18-35 x 4.2K (117 us, 177 in runs),
-// the first, lower one lets 20 nodes x 4K be cut (31.4 us; 36.1 at 0.15).
+// joined, and one beyond a round of the CTAs. Fitted on 35 workloads of 1 to 230 nodes, within 2 % over a wide
+// range of prices for most. Where it shows, at these and at (4, .04, .08): 3 x 3 nodes x 2K keys 17.4 / 19.1 us,
+// 64 x 2 x 4K 81.8 / 85.4, lists 1 x 16 x 2048 22.5 / 24.0; lower ones cut too much (1 x 1 x 8K 17.6, 20.4 at .01).
 struct TreePrice {
     float item, part, more;
 };
-constexpr TreePrice TA_PRICE = {4.f, 0.04f, 0.08f};
+constexpr TreePrice TA_PRICE = {4.f, 0.02f, 0.06f};
 
 template <bool SEL>
 struct TaLayout {
