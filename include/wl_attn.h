@@ -509,7 +509,7 @@ typedef struct wl_tree_attn_io {
     int32_t  ctx_type;             /* WL_F32 or WL_BF16                              */
     const int32_t* sel_in;         /* consumer: device [n_nodes, sel_stride]         */
     const int32_t* sel_n_in;       /* consumer: device [n_nodes], or NULL -> sel_n   */
-    int32_t  sel_n;
+    int32_t  sel_n;                /* with sel_n_in: larger counts end here (0: at sel_stride) */
     int64_t  sel_stride;
     void*    ctx;                  /* out: [n_nodes, n_heads, kv_lora]               */
     float*   lse;                  /* out, optional: fp32 [n_nodes, n_heads]         */

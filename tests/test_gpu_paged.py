@@ -138,6 +138,12 @@ def test_plan_flags_bad_lengths_and_overflowing_rows():
     bad_word()
 
 
+def test_plan_of_a_table_without_rows():
+    e = torch.empty(0, dtype=torch.int32, device="cuda")
+    got = P.page_plan(e, e, torch.zeros(0, 3, dtype=torch.int32, device="cuda"), e, i32([0, 1]), i32([2]), 8, 3)
+    assert cpu(got["cu"]).tolist() == [0] and cpu(got["slot"]).tolist() == [-1] * 3
+
+
 def test_plan_of_no_requests():
     e = torch.empty(0, dtype=torch.int32, device="cuda")
     got = P.page_plan(e, e, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), e, i32([0, 1]), i32([2]), 8, 3)
@@ -432,6 +438,15 @@ def test_selected_keys(ctx, nodes, page, k, dtype):
     t.check(got, sel=sel)
 
 
+def test_lists_end_at_the_slice_that_holds_them():
+    """A list tensor that is a slice of a wider one: counts above its width do not reach the columns behind it."""
+    t = Trees([400, 90], [3, 2], 16, seed=21)
+    rng = np.random.default_rng(21)
+    wide = np.stack([rng.permutation(90)[:60] for _ in range(5)]).astype(np.int32)
+    got = t.call(sel_in=i32(wide)[:, 10:37], sel_n_in=i32([27, 28, 60, 10 ** 9, 5]))
+    t.check(got, sel=[wide[r, 10:10 + min(27, c)] for r, c in enumerate([27, 28, 60, 10 ** 9, 5])])
+
+
 def test_selecting_everything_is_the_dense_result():
     t = Trees([500, 64], [5, 2], 16, seed=11)
     every = np.tile(np.arange(505, dtype=np.int32), (7, 1))
@@ -700,3 +715,11 @@ def test_a_request_without_pages_neither_reads_nor_moves_others_rows():
     P.tree_commit(P.LayerCaches([kv]), i32([20, 14]), plan["cu"], par, tok, tgt)
     bad_word()
     assert torch.equal(pool, was)
+
+
+def test_layers_of_one_commit_share_the_whole_table():
+    kv = torch.zeros(32, 576, dtype=torch.bfloat16, device="cuda")
+    wide = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    a, b = (P.PagedKV.packed(kv, 8, t) for t in (wide[:, :2], wide))
+    with pytest.raises(ValueError, match="share one block table"):
+        P.LayerCaches([a, b])

@@ -58,6 +58,7 @@ def test_tree_attention_refuses(kw):
 def test_tree_attention_accepts_nothing_to_do_and_refuses_what_it_would_read():
     assert attn(attn_io(batch=0, ctx_len=None, cu_nodes=None)) == OK  # no requests
     assert attn(attn_io(n_nodes=0)) == OK
+    assert attn(attn_io(batch=0, ctx_len=None, block_table=None)) == OK
     assert attn(attn_io(batch=2, q_abs=None)) == ARG
     assert attn(attn_io(batch=2, q_abs=FAKE + 2)) == ARG
     assert attn(attn_io(batch=2, ctx=None)) == ARG
@@ -95,6 +96,7 @@ def test_page_release_refuses():
         a[i] = bad
         assert lib().wl_page_release(*a, None) == ARG, i
     assert lib().wl_page_release(0, *good[1:], None) == OK
+    assert lib().wl_page_release(0, None, None, 4, 4, None, None, 10, None, None) == OK  # no requests, no table
 
 
 def commit_io(**kw):

@@ -58,7 +58,7 @@ struct TreeParams {
     const int* sel;          // null: every key
     long long sel_stride;
     const int* sel_n_dev;
-    int sel_n;
+    int sel_n;  // entries of a list, or with sel_n_dev at most
     float scale_log2;
     void* ctx;
     int ctx_bf16;
@@ -158,8 +158,7 @@ static_assert(TA_MAX_BATCH * 8 <= TaLayout<false>::OFF_P, "schedule table");
 
 // Keys of a row's list (clamped to the list's room).
 __device__ __forceinline__ int tree_list_n(const TreeParams& p, int r) {
-    const int n = p.sel_n_dev ? __ldg(p.sel_n_dev + r) : p.sel_n;
-    return (int)min((long long)max(n, 0), p.sel_stride);
+    return p.sel_n_dev ? max(0, min(__ldg(p.sel_n_dev + r), p.sel_n)) : p.sel_n;
 }
 // Key tiles of a request's nodes (at least one).
 template <bool SEL>

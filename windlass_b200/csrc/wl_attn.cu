@@ -1249,7 +1249,7 @@ int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* 
 static int check_pages(int32_t batch, int32_t page_size, int32_t n_pages, const int32_t* table, int64_t table_stride,
                        int32_t max_pages) {
     if (batch < 0 || page_size <= 0 || n_pages <= 0 || (int64_t)page_size * n_pages > INT32_MAX) return WL_ERR_ARG;
-    if (!table || max_pages <= 0 || table_stride < max_pages) return WL_ERR_ARG;
+    if ((!table && batch > 0) || max_pages <= 0 || table_stride < max_pages) return WL_ERR_ARG;
     return WL_OK;
 }
 
@@ -1420,7 +1420,9 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     p.sel = io->mode == WL_MODE_CONSUMER ? io->sel_in : nullptr;
     p.sel_stride = io->sel_stride;
     p.sel_n_dev = io->sel_n_in;
-    p.sel_n = io->sel_n;
+    // entries of a list that may be read at all
+    const int64_t room = io->sel_n > 0 && io->sel_n < io->sel_stride ? io->sel_n : io->sel_stride;
+    p.sel_n = io->sel_n_in ? (int)(room < INT32_MAX ? room : INT32_MAX) : io->sel_n;
     p.scale_log2 = cfg->softmax_scale * 1.4426950408889634f;
     p.ctx = io->ctx;
     p.ctx_bf16 = io->ctx_type == WL_BF16;

@@ -177,7 +177,7 @@ def mla_tree_attn(cfg: AttnCfg, kv: PagedKV, q_abs: torch.Tensor, ctx_len: torch
     ancestors by ``parent`` [n] (int32, index within the request, -1 for a root), or the
     nodes of ``mask`` [n] (int64 bit masks), or nodes 0..i (neither given: a chain; one node
     is plain decode). ``sel_in`` [n, k] int32 (with counts ``sel_n_in`` [n]) narrows each
-    row to its own list of unique positions, in any order. Returns ctx [n, 64, 512] of
+    row to its own list of unique positions, in any order (counts above k end there). Returns ctx [n, 64, 512] of
     ``out_dtype`` (float32 or bfloat16) and lse [n, 64] fp32 — the given tensors, where
     given; rows behind the last request are not written."""
     dev = q_abs.device
@@ -247,7 +247,8 @@ class LayerCaches:
         first = kvs[0]
         rows = first.c_kv.shape[0]
         for kv in kvs:
-            if kv.page_size != first.page_size or kv.block_table.data_ptr() != first.block_table.data_ptr():
+            t, u = kv.block_table, first.block_table
+            if kv.page_size != first.page_size or t.data_ptr() != u.data_ptr() or t.shape != u.shape or t.stride() != u.stride():
                 raise ValueError("the layers must share one block table and page size")
             if kv.c_kv.device != first.c_kv.device:
                 raise ValueError("the layers must be on one device")
