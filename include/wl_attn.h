@@ -487,14 +487,17 @@ int wl_cache_append_paged(const wl_attn_cfg* cfg, const wl_cache_append_io* io, 
  * its ancestors by `parent` (parent[row] = index of the parent within the
  * request, -1 for a root) and itself, or, with both NULL, nodes 0..i (a chain).
  * WL_MODE_CONSUMER narrows this to the row's own list sel_in[row] of unique
- * positions (any order; entries that the row may not see are dropped);
+ * positions (any order; entries that the row may not see are dropped, a
+ * position named twice counts twice);
  * WL_MODE_DENSE takes every key it sees. Rows that see nothing get ctx = 0 and
  * lse = -inf; rows of no request (behind cu_nodes[batch]) are left as they are.
  * Keys that a row does not see never reach it, whatever their rows hold.
  * A request whose numbers are out of range (more than 64 nodes, rows outside
  * [0, n_nodes), ctx_len + nodes above cfg->T_max or its table), and a table
  * entry outside the pool, set the device error word; the request's rows are
- * left as they are, the page's keys are left out. ctx is fp32 or bf16; P enters the P.V product
+ * left as they are, the page's keys are left out. The width of the table
+ * (max_pages) is all that the host knows of the lengths: one that is no wider
+ * than they need lets a call choose its kernel well. ctx is fp32 or bf16; P enters the P.V product
  * in bf16 (as in wl_attn_decode), its sum in fp32 before that rounding. */
 typedef struct wl_tree_attn_io {
     int32_t batch;

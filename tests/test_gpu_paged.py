@@ -172,7 +172,9 @@ def test_release_then_plan_hands_the_pages_out_again(B):
 # ---- attention -------------------------------------------------------------------------------
 
 class Trees:
-    """A pool, block tables and trees of given context lengths and node counts."""
+    """A pool, block tables and trees of given context lengths and node counts. ``wide``: the table has room for
+    long requests, with which trees of many nodes are worked on by pairs of CTAs whatever their lengths."""
+    wide = True
 
     def __init__(self, ctx, nodes, page, seed=0, row=576, split=False, spread=1.0, spare_rows=0, pages=None):
         rng = np.random.default_rng(seed)
@@ -201,7 +203,8 @@ class Trees:
         self.masks = R.tree_masks(self.parent, self.cu)
 
     def kv(self):
-        return P.PagedKV(self.c_kv, self.k_rot, self.page, i32(self.table))
+        room = 20480 // self.page + 1 if self.wide else 0
+        return P.PagedKV(self.c_kv, self.k_rot, self.page, i32(np.pad(self.table, ((0, 0), (0, room)), constant_values=-7)))
 
     def call(self, **kw):
         kw.setdefault("parent", i32(self.parent))
@@ -242,8 +245,10 @@ CASES = [
 
 @pytest.mark.parametrize("ctx,nodes,page", CASES)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_tree_attention_matches_64_bits(ctx, nodes, page, dtype):
+@pytest.mark.parametrize("wide", [True, False])
+def test_tree_attention_matches_64_bits(ctx, nodes, page, dtype, wide):
     t = Trees(ctx, nodes, page, seed=len(ctx) + page)
+    t.wide = wide
     t.check(t.call(out_dtype=dtype))
 
 
@@ -294,10 +299,12 @@ def test_many_requests_and_long_contexts():
 
 
 @pytest.mark.parametrize("B,lo,hi", [(30, 8, 12), (60, 2, 4), (61, 1, 9), (200, 1, 3)])
-def test_more_work_than_a_round_of_the_gpu(B, lo, hi):
+@pytest.mark.parametrize("wide", [True, False])
+def test_more_work_than_a_round_of_the_gpu(B, lo, hi, wide):
     """Every CTA (pair) takes several pieces of work one after the other, of all lengths."""
     rng = np.random.default_rng(B)
     t = Trees(rng.integers(0, 400, B).tolist(), rng.integers(lo, hi, B).tolist(), 16 if B % 2 else 64, seed=B)
+    t.wide = wide
     got = t.call()
     t.check(got)
     for _ in range(5):
@@ -321,8 +328,10 @@ def test_all_64_bits_of_a_mask():
 
 
 @pytest.mark.parametrize("nodes", [[13, 64], [64, 1]])
-def test_masks_of_many_nodes(nodes):
+@pytest.mark.parametrize("wide", [True, False])
+def test_masks_of_many_nodes(nodes, wide):
     t = Trees([0, 70], nodes, 16, seed=21)
+    t.wide = wide
     rng = np.random.default_rng(21)
     masks = [int(rng.integers(0, 1 << 62)) & int(rng.integers(0, 1 << 62)) | int(rng.integers(0, 4)) << 62 for _ in range(t.n)]
     masks[0] = masks[3] = 0  # request 0 has no context: these rows see nothing
@@ -445,6 +454,20 @@ def test_lists_end_at_the_slice_that_holds_them():
     wide = np.stack([rng.permutation(90)[:60] for _ in range(5)]).astype(np.int32)
     got = t.call(sel_in=i32(wide)[:, 10:37], sel_n_in=i32([27, 28, 60, 10 ** 9, 5]))
     t.check(got, sel=[wide[r, 10:10 + min(27, c)] for r, c in enumerate([27, 28, 60, 10 ** 9, 5])])
+
+
+def test_a_position_named_twice_counts_twice():
+    t = Trees([50], [2], 16, seed=25)
+    got = t.call(sel_in=i32([[7, 9, 7], [49, 3, 3]]))
+    q, rows = t.q.float().cpu().numpy().astype(np.float64), t.rows().astype(np.float64)
+    for r, x in enumerate(([7, 9, 7], [49, 3, 3])):
+        k = rows[[t.table[0, p // 16] * 16 + p % 16 for p in x]]
+        e = np.exp(q[r] @ k.T * SCALE)
+        p = e / e.sum(1, keepdims=True)
+        ref, spread = p @ k[:, :512], p @ np.abs(k[:, :512])
+        # P to bf16 and 2 DS of unit-size q and k, as above
+        assert np.all(np.abs(cpu(got["ctx"])[r] - ref) <= (2.0 ** -8 + 4e-4) * spread)
+        assert np.abs(cpu(got["lse"])[r] - np.log(e.sum(1))).max() < 4e-4
 
 
 def test_selecting_everything_is_the_dense_result():

@@ -1421,8 +1421,8 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     p.sel_stride = io->sel_stride;
     p.sel_n_dev = io->sel_n_in;
     // entries of a list that may be read at all
-    const int64_t room = io->sel_n > 0 && io->sel_n < io->sel_stride ? io->sel_n : io->sel_stride;
-    p.sel_n = io->sel_n_in ? (int)(room < INT32_MAX ? room : INT32_MAX) : io->sel_n;
+    const int64_t entries = io->sel_n > 0 && io->sel_n < io->sel_stride ? io->sel_n : io->sel_stride;
+    p.sel_n = io->sel_n_in ? (int)(entries < INT32_MAX ? entries : INT32_MAX) : io->sel_n;
     p.scale_log2 = cfg->softmax_scale * 1.4426950408889634f;
     p.ctx = io->ctx;
     p.ctx_bf16 = io->ctx_type == WL_BF16;
@@ -1439,11 +1439,17 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     p.box_rows = (kv.page_size & -kv.page_size) < wl::TA_TILE ? (kv.page_size & -kv.page_size) : wl::TA_TILE;
     wl::TreeMaps tm{};
     if (int e = encode_q_map(&tm.q, io->q_abs, io->n_nodes)) return e;
-    // Two nodes of a request at a time, by CTA pairs, for trees of six and more nodes; one at a time for smaller
-    // ones (a lone or last odd node leaves half of a pair's rows empty, and with little work the pair's longer
-    // start and end show) and for lists (a list per node). One at a time / pairs, us: 20 nodes of 4 requests, 4K
-    // keys 31 / 35; 40 of 17, 13K 94 / 99; 90 of 15, 2.6K 65 / 54; 92 of 8, 16K 208 / 191; 394 of 16, 32K 1600 / 1318.
-    const bool pairs = !p.sel && io->n_nodes >= 12 && (int64_t)io->n_nodes >= 6 * (int64_t)io->batch;
+    // Two nodes of a request at a time, by CTA pairs, when there is enough to do; one at a time for small trees (a
+    // lone or last odd node leaves half of a pair's rows empty), for few keys (the pair's start and end take 8 us
+    // longer) and for lists (a list per node). The lengths are on the device, so the keys are counted as if every
+    // row's request filled its table row. One at a time / pairs, us:
+    //   by keys      20 nodes x 4K 28 / 37; 16 x 8K 36 / 45; 64 x 1K 30 / 36; 45 x 4K 39 / 42; 57 x 3K 38 / 41;
+    //                64 x 4K 59 / 56; 32 x 8K 56 / 51; 35 x 8K 58 / 53; 12 x 60K 120 / 115; 16 x 30K 84 / 72;
+    //                92 x 16K 190 / 168; 394 x 32K 1625 / 1240
+    //   by tree      46 of 16 requests x 8K 67 / 67; 40 of 17 x 13K 94 / 99; 90 of 15 x 2.6K 65 / 55; 11 of 4 x 30K 52 / 59
+    const int64_t room = (int64_t)kv.max_pages * kv.page_size, most = room < cfg->T_max ? room : cfg->T_max;
+    const bool pairs = !p.sel && io->n_nodes >= 12 && (int64_t)io->n_nodes >= 6 * (int64_t)io->batch &&
+                       (int64_t)io->n_nodes * most >= 240 * 1024;
     const uint32_t out_rows = pairs ? 32 : 16;  // a warp's rows
     if (int e = encode_out_map(&tm.part, p.o_part, parts, false, out_rows)) return e;
     if (int e = encode_out_map(&tm.out, io->ctx, io->n_nodes, p.ctx_bf16, out_rows)) return e;

@@ -70,7 +70,8 @@ class PagedKV:
     stride that keeps them 16-byte aligned), pages of ``page_size`` rows (a multiple of
     8), ``block_table`` [batch, max_pages] int32. Slots past the last whole page are
     not used. ``packed(kv)`` splits a [slots, 576] tensor. The views are taken when
-    the object is made; their contents, the table's included, may change freely."""
+    the object is made; their contents, the table's included, may change freely. A table no
+    wider than the requests need lets ``mla_tree_attn`` choose its kernel well."""
     c_kv: torch.Tensor
     k_rot: torch.Tensor
     page_size: int
