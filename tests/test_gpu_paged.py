@@ -746,3 +746,15 @@ def test_layers_of_one_commit_share_the_whole_table():
     a, b = (P.PagedKV.packed(kv, 8, t) for t in (wide[:, :2], wide))
     with pytest.raises(ValueError, match="share one block table"):
         P.LayerCaches([a, b])
+
+
+def test_append_stays_inside_the_smallest_pool():
+    """Keys with fewer scales than rows: the slots behind the scales are flagged, and neither is written."""
+    keys = A.IndexKeys(torch.zeros(32, 128, dtype=torch.uint8, device="cuda"), torch.zeros(32, device="cuda")[:16])
+    one, zero = torch.ones(2, 32, device="cuda"), torch.zeros(2, 32, device="cuda")
+    kn = torch.ones(128, device="cuda", dtype=torch.bfloat16)
+    raw = torch.randn(2, 128, device="cuda")
+    P.cache_append_paged(A.glm52_cfg(8), i32([3, 20]), one, zero, keys=keys, k_raw=raw, k_norm_w=kn, k_norm_b=kn)
+    bad_word()
+    assert torch.nonzero(keys.scale).flatten().tolist() == [3]
+    assert torch.nonzero(keys.keys.sum(1)).flatten().tolist() == [3]

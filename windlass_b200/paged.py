@@ -45,12 +45,15 @@ def _i32(t: torch.Tensor, name: str, dev: torch.device, numel: int | None = None
     return t.data_ptr()
 
 
-def _table(t: torch.Tensor, batch: int, dev: torch.device) -> int:
+def _table(t: torch.Tensor, batch: int, dev: torch.device) -> tuple[int, int, int]:
+    """(address, row stride, entries a row) of a block table of at least ``batch`` rows."""
     if t.dtype != _I32 or t.dim() != 2 or t.device != dev:
         raise ValueError(f"block_table must be a 2-D int32 tensor on {dev}")
-    if t.shape[0] < batch or (t.shape[1] > 1 and t.stride(1) != 1) or (batch > 1 and t.stride(0) < t.shape[1]):
+    rows, width = t.shape
+    row, col = t.stride()
+    if rows < batch or (width > 1 and col != 1) or (batch > 1 and row < width):
         raise ValueError(f"block_table must have {batch} rows of consecutive entries")
-    return t.data_ptr()
+    return t.data_ptr(), row if batch > 1 else max(width, 1), width
 
 
 def _call(dev: torch.device, fn, *args) -> int:
@@ -93,8 +96,7 @@ class PagedKV:
         if self.page_size <= 0 or self.page_size % 8 or self.n_pages <= 0:
             raise ValueError("page_size must be a multiple of 8 that the pool holds at least once")
         lat = LatentKV(ckv.unsqueeze(0), krt.unsqueeze(0)).c()
-        self._c = PagedKVC(lat, self.page_size, self.n_pages, _table(t, t.shape[0], ckv.device), t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1),
-                           t.shape[1])
+        self._c = PagedKVC(lat, self.page_size, self.n_pages, *_table(t, t.shape[0], ckv.device))
 
     def c(self) -> PagedKVC:
         return self._c
@@ -119,7 +121,8 @@ def page_plan(ctx_len: torch.Tensor, n_new: torch.Tensor, block_table: torch.Ten
     B, T = ctx_len.numel(), int(n_tokens)
     c, n, held, nf = (_i32(ctx_len, "ctx_len", dev), _i32(n_new, "n_new", dev, B), _i32(n_held, "n_held", dev, B),
                       _i32(n_free, "n_free", dev, 1))
-    table, free = _table(block_table, B, dev), _i32(free_list, "free_list", dev)
+    table, stride, width = _table(block_table, B, dev)
+    free = _i32(free_list, "free_list", dev)
     if T < 0:
         raise ValueError("n_tokens must not be negative")
     # one allocation: slot, pos, seq [T], cu [B + 1], short [B] and, unless in place, n_held [B] and n_free [1]
@@ -127,11 +130,11 @@ def page_plan(ctx_len: torch.Tensor, n_new: torch.Tensor, block_table: torch.Ten
     out = torch.empty(sum(sizes), dtype=_I32, device=dev)
     o = out.data_ptr()
     short = o + 4 * (3 * T + B + 1)
-    io = _lib.PagePlanIO(B, T, page_size, free_list.numel(), c, n, table, block_table.stride(0) if B > 1 else max(block_table.shape[1], 1),
-                         block_table.shape[1], held, held if in_place else short + 4 * B, free, nf,
-                         nf if in_place else short + 8 * B, o + 12 * T, short, o, o + 4 * T, o + 8 * T)
+    io = _lib.PagePlanIO(B, T, page_size, free_list.numel(), c, n, table, stride, width, held,
+                         held if in_place else short + 4 * B, free, nf, nf if in_place else short + 8 * B, o + 12 * T,
+                         short, o, o + 4 * T, o + 8 * T)
     check(_call(dev, lib().wl_page_plan, C.byref(io)), "wl_page_plan")
-    parts = out.split_with_sizes(sizes)
+    parts = torch.unsafe_split_with_sizes(out, sizes)  # (integers: no gradient to track, and `out` ends here)
     return dict(slot=parts[0], pos=parts[1], seq=parts[2], cu=parts[3], short=parts[4],
                 n_held=n_held if in_place else parts[5], n_free=n_free if in_place else parts[6])
 
@@ -142,9 +145,7 @@ def page_release(done: torch.Tensor, block_table: torch.Tensor, n_held: torch.Te
     place (``wl_page_release``)."""
     dev = done.device
     B = done.numel()
-    args = (B, _i32(done, "done", dev), _table(block_table, B, dev),
-            block_table.stride(0) if B > 1 else max(block_table.shape[1], 1), block_table.shape[1],
-            _i32(n_held, "n_held", dev, B), _i32(free_list, "free_list", dev), free_list.numel(),
+    args = (B, _i32(done, "done", dev), *_table(block_table, B, dev), _i32(n_held, "n_held", dev, B), _i32(free_list, "free_list", dev), free_list.numel(),
             _i32(n_free, "n_free", dev, 1))
     check(_call(dev, lib().wl_page_release, *args), "wl_page_release")
 
@@ -154,10 +155,10 @@ def cache_append_paged(cfg: AttnCfg, slot: torch.Tensor, cos: torch.Tensor, sin:
     """``cache_append`` into pools: token i goes to row ``slot[i]`` (``page_plan``'s slots), -1
     is skipped. ``keys`` is the owner layer's index pool (keys [slots, 128], scale
     [slots]); the other arguments are ``cache_append``'s."""
-    pools = [t for t in (kv.c_kv if kv is not None else None, keys.keys if keys is not None else None) if t is not None]
+    pools = ([kv.c_kv] if kv is not None else []) + ([keys.keys, keys.scale] if keys is not None else [])
     if not pools:
         raise ValueError("cache_append_paged needs kv or keys")
-    if keys is not None and keys.keys.dim() != 2:
+    if keys is not None and (keys.keys.dim() != 2 or keys.scale.dim() != 1):
         raise ValueError("index pools must be [slots, 128] with scales [slots]")
     io, hold = cache_append_io(slot, cos, sin, kv=None if kv is None else kv.latent(), keys=keys, **kw)
     n_slots = min(t.shape[0] for t in pools)
@@ -182,8 +183,9 @@ def mla_tree_attn(cfg: AttnCfg, kv: PagedKV, q_abs: torch.Tensor, ctx_len: torch
     ``out_dtype`` (float32 or bfloat16) and lse [n, 64] fp32 — the given tensors, where
     given; rows behind the last request are not written."""
     dev = q_abs.device
-    n, B = q_abs.shape[0], ctx_len.numel()
-    if q_abs.dtype != torch.bfloat16 or tuple(q_abs.shape[1:]) != (N_HEADS, D_QK):
+    shape, B = q_abs.shape, ctx_len.numel()
+    n = shape[0] if shape else 0
+    if q_abs.dtype != torch.bfloat16 or len(shape) != 3 or shape[1] != N_HEADS or shape[2] != D_QK:
         raise ValueError("q_abs must be bf16 [n, 64, 576]")
     if kv.c_kv.device != dev:
         raise ValueError(f"the pool must be on {dev}, got {kv.c_kv.device}")
@@ -296,7 +298,7 @@ def tree_commit(layers: LayerCaches, ctx_len: torch.Tensor, cu_nodes: torch.Tens
                            kv.page_size, layers.n_pages, kv.block_table, kv.table_stride, kv.max_pages,
                            len(layers.kvs), layers._latent, layers._index, acc, path, acc + 4 * B, acc + 8 * B)
     check(_call(dev, lib().wl_tree_commit, C.byref(cfg if cfg is not None else _default_cfg()), C.byref(io)), "wl_tree_commit")
-    parts = out.split_with_sizes(sizes)
+    parts = torch.unsafe_split_with_sizes(out, sizes)
     return dict(n_accept=parts[1], path=parts[0].view(B, TREE_MAX), next=parts[2], ctx_len=parts[3])
 
 
