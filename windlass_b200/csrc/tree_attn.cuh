@@ -184,10 +184,11 @@ __device__ __forceinline__ int div_near(int x, int c, float inv) {
 // Tiles per item, from the lengths: a request's nodes are cut into the fewest
 // equal runs of at most C tiles, with C = ceil(longest / s) for 64 values of s.
 // The CTAs take the items in order, forth and back (item_of); with the longest
-// requests first (up to 32 requests are sorted) full rounds balance out, so a
-// choice costs the mean of its full rounds plus the longest item of the last one,
-// plus a write and a read per partial: within 5 % of the best of all choices on
-// 26 drawn workloads. The cheapest that fits the workspace is taken, the fewest
+// runs first (up to 32 requests are sorted, by their tiles for the choice and by
+// their runs' for the walk: 4 requests, 177 nodes x 10K 244 -> 201 us, 25, 512 x 1.5K
+// 131 -> 116) full rounds balance out, so a choice costs the mean of its full
+// rounds plus the longest item of the last one, plus a write and a read per
+// partial: within 5 % of the best of all choices on 26 drawn workloads. The cheapest that fits the workspace is taken, the fewest
 // runs among equals. Every CTA computes the same choice, all its threads sharing
 // the sums (64 candidates x 3 thirds of the requests); the producer warp, which
 // alone needs it, ends with C. tab: (nodes, tiles) of each request; acc: 4 x 3 x 64.
@@ -200,14 +201,21 @@ struct TreeCost {
 __device__ __forceinline__ float tree_candidate(int c) {
     return c < 32 ? 1.f + 0.25f * c : c < 48 ? 9.f + (c - 32) : 24.f + 8.5f * (c - 47);
 }
-__device__ __forceinline__ int tree_run_tiles(int longest, float s) { return max(1, (int)ceilf(__fdividef((float)longest, s))); }
+// The tiles a run then has at most. Of eight and more requests none is cut into more than 24 runs with profit: there
+// the lengths of the first 16 take the place of the last candidates, so that all longer ones are cut and no other
+// (8 requests, 92 nodes x 16K 176 -> 167 us; 12, 479 x 17K 751 -> 725; 23, 311 x 6K 204 -> 197).
+__device__ __forceinline__ int tree_run_tiles(int c, int longest, const int2* tab, int batch) {
+    if (c >= 48 && batch >= 8)
+        return max(max(1, tab[min(c - 48, batch - 1)].y), (longest + TA_MAX_SPLIT - 1) / TA_MAX_SPLIT);
+    return max(1, (int)ceilf(__fdividef((float)longest, tree_candidate(c))));
+}
 
 template <int PER>  // nodes an item takes
 __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* tab, int longest, TreeCost* acc, int G, TreePrice price,
                                              int last_warp = TA_LOAD_WARP) {
     const int cand = threadIdx.x % TA_CANDS, grp = threadIdx.x / TA_CANDS;
     const int per = (p.batch + 2) / 3, b0 = min(grp * per, p.batch), b1 = min(b0 + per, p.batch);
-    const int C = tree_run_tiles(longest, tree_candidate(cand));
+    const int C = tree_run_tiles(cand, longest, tab, p.batch);
     const float inv = __fdividef(1.f, (float)C);
     const bool mine = threadIdx.x < TA_SCHED_THREADS;
     if (mine) {
@@ -243,7 +251,8 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
     __syncthreads();
     if ((int)threadIdx.x / 32 != last_warp) return 0;
     const int lane = threadIdx.x & 31;
-    float best = 3e38f, best_s = 1.f;
+    float best = 3e38f;
+    int best_c = max(1, longest);
     const float inv_g = __fdividef(1.f, (float)G);
 #pragma unroll
     for (int c = lane; c < TA_CANDS; c += 32) {
@@ -253,19 +262,19 @@ __device__ __forceinline__ int tree_schedule(const TreeParams& p, const int2* ta
                            (float)max(0, n_parts - G * PER) * (price.more - price.part);
         if (n_parts <= p.parts_max && cost < best) {
             best = cost;
-            best_s = tree_candidate(c);
+            best_c = tree_run_tiles(c, longest, tab, p.batch);
         }
     }
 #pragma unroll 1
     for (int o = 16; o > 0; o >>= 1) {
         const float c = __shfl_xor_sync(0xffffffffu, best, o);
-        const float t = __shfl_xor_sync(0xffffffffu, best_s, o);
-        if (c < best || (c == best && t < best_s)) {
+        const int t = __shfl_xor_sync(0xffffffffu, best_c, o);
+        if (c < best || (c == best && t > best_c)) {
             best = c;
-            best_s = t;
+            best_c = t;
         }
     }
-    return tree_run_tiles(longest, best_s);
+    return best_c;
 }
 // Worker me's item of round k: the G workers take them forth and back.
 __device__ __forceinline__ int item_of(int k, int me, int G) { return k * G + ((k & 1) ? G - 1 - me : me); }
@@ -290,9 +299,9 @@ struct TreeWalk {
             tiles = n > 0 ? tree_tiles<SEL>(p, s) : 0;
         }
     }
-    __device__ void sort() {  // longest first (a single block only), by a bitonic network
+    __device__ void sort(int by) {  // largest first (a single block only), by a bitonic network
         const int lane = threadIdx.x & 31;
-        unsigned key = (unsigned)tiles * 32u + (unsigned)(31 - lane);  // tiles < 2^26
+        unsigned key = (unsigned)by * 32u + (unsigned)(31 - lane);  // by < 2^26
 #pragma unroll 1
         for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll 1
@@ -308,9 +317,12 @@ struct TreeWalk {
         ctx = __shfl_sync(0xffffffffu, ctx, from);
         tiles = __shfl_sync(0xffffffffu, tiles, from);
     }
-    __device__ void count() {  // items and parts of the loaded block
+    __device__ int run_len() const {
         const int r = div_near(tiles + C - 1, C, __fdividef(1.f, (float)C));
-        len = r > 1 ? div_near(tiles + r - 1, r, __fdividef(1.f, (float)r)) : max(tiles, 1);
+        return r > 1 ? div_near(tiles + r - 1, r, __fdividef(1.f, (float)r)) : max(tiles, 1);
+    }
+    __device__ void count() {  // items and parts of the loaded block
+        len = run_len();
         runs = div_near(tiles + len - 1, len, __fdividef(1.f, (float)len));  // <= r: no run is empty
         const int it = (n + PER - 1) / PER * runs, pt = runs > 1 ? n * runs : 0;
         int si = it, sp = pt;
@@ -519,7 +531,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
         walk.b0 = walk.item0 = walk.part0 = 0;
         walk.load(p);
         if (!many) {
-            if (p.batch > 1) walk.sort();
+            if (p.batch > 1) walk.sort(walk.tiles);
             if (lane < p.batch) tab[lane] = make_int2(walk.n, walk.tiles);
             if (lane == 0) *longest_sh = walk.tiles;
         }
@@ -532,6 +544,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
     }
 
     if (warp == TA_LOAD_WARP) {  // the producer, or the first gather warp
+        if (p.batch > 1 && !many) walk.sort(walk.run_len());
         walk.count();
         if (blockIdx.x == gridDim.x - 1) tree_table(p, walk);
     }

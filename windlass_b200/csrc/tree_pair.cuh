@@ -44,7 +44,9 @@ constexpr int TP_UNITS = 6;   // score CTA: [even, odd][3] thirds of a tile (64 
 constexpr int TP_HALVES = 4;  // value CTA: [even, odd][2] halves of a tile (64 keys x 256 columns)
 constexpr int TP_P = 4;       // value CTA: tiles of P (score CTA: on their way), tile & 3
 constexpr uint32_t TP_TM_S = 384;  // score columns in tensor memory (the queries take [0, 288))
-constexpr TreePrice TP_PRICE = {6.f, 0.12f, 0.2f};  // (0.8 us a tile; see TA_PRICE)
+// (0.8 us a tile; see TA_PRICE. At these and at (6, .12, .2): 9 requests, 109 nodes x 9K 126 / 144 us, 12, 74 x 13K
+// 121 / 128, 8, 92 x 16K 166 / 169; 20, 235 x 3K 95 / 92.)
+constexpr TreePrice TP_PRICE = {6.f, 0.03f, 0.06f};
 
 struct TpLayout {
     static constexpr uint32_t CHUNK = TA_TILE * 128;          // 8 KB: 64 keys x 64 columns
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
         walk.b0 = walk.item0 = walk.part0 = 0;
         walk.load(p);
         if (!many) {
-            if (p.batch > 1) walk.sort();
+            if (p.batch > 1) walk.sort(walk.tiles);
             if (warp == TP_LOAD_WARP && lane < p.batch) tab[lane] = make_int2(walk.n, walk.tiles);
             if (warp == TP_LOAD_WARP && lane == 0) *longest_sh = walk.tiles;
         }
@@ -239,6 +241,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
     };
     if (loads) {
         // ---------------- loads: even or odd tiles ----------------
+        if (p.batch > 1 && !many) walk.sort(walk.run_len());
         walk.count();
         const int which = warp - TP_LOAD_WARP;
         if (score && me == G - 1 && which == 0) tree_table(p, walk);
