@@ -408,7 +408,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                 tmem_ld64(tmem + lanes + TP_TM_S + (uint32_t)(s * TA_TILE), sv);
                 tc_fence_before();
                 mbar_arrive(sfree + s);
-                const unsigned long long bits = tree_tile_mask(see, t.pos0 + i * TA_TILE, t.ctx) & ~lost_sh[gt & 7];
+                const unsigned long long lost = lost_sh[gt & 7];
+                const unsigned long long bits = tree_tile_mask(see, t.pos0 + i * TA_TILE, t.ctx) & ~lost;
                 if (flip) {
 #pragma unroll
                     for (int j = 0; j < 64; ++j) sv[j] = -sv[j];
@@ -445,8 +446,9 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                     }
                     sts_v4(prow + (uint32_t)((c ^ r) & 7) * 16u, make_uint4(w[0], w[1], w[2], w[3]));
                 }
-                // O moves to the new maximum only after the item's first tile
-                alpha_sh[128 * pb + r] = i == 0 || m_new == m_run ? 1.f : alpha;
+                // O moves to the new maximum only after the item's first tile; the sign tells of keys lost to bad pages
+                const float factor = i == 0 || m_new == m_run ? 1.f : alpha;
+                alpha_sh[128 * pb + r] = lost != 0 ? -factor : factor;
                 l_run = l_run * (m_mine == -INFINITY ? 0.f : exp2_ftz(m_mine - m_new)) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
                 m_mine = m_new;
                 fence_proxy_async_smem();  // the copies read this warp's writes
@@ -526,11 +528,14 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                 const int pb = gt & 3, v = 2 * (gt & 1);
                 if (!(ok = mbar_wait_fast(pfull + pb, (uint32_t)(gt >> 2) & 1u, 85))) break;
                 if (tid == 0) mbar_expect_tx(pfull + pb, L::P + 512);  // for the P of four tiles on
-                const float alpha = alpha_sh[128 * pb + r];
-                // (the loader's word on the tile is read once its keys are here)
-                if (!(ok = mbar_wait_fast(vfull + v, (uint32_t)(gt >> 1) & 1u, 86) && mbar_wait_fast(vfull + v + 1, (uint32_t)(gt >> 1) & 1u, 86))) break;
-                const unsigned long long lost = lost_sh[gt & 7];
-                if (pos + TA_TILE > t.ctx || lost != 0) {  // rows that not both nodes see
+                const float alpha = fabsf(alpha_sh[128 * pb + r]);
+                if (pos + TA_TILE > t.ctx || signbit(alpha_sh[128 * pb + r])) {  // rows that not both nodes see
+                    // These warps run ahead of the values (waiting for them in every tile cost 2 to 4 %), so
+                    // the space's use before comes first: its barrier's phase could be taken for this one's. The
+                    // loader's word on the tile is read once its keys are here.
+                    if (gt >= 2 && !(ok = pv_done(gt - 2, 84))) break;
+                    if (!(ok = mbar_wait_fast(vfull + v, (uint32_t)(gt >> 1) & 1u, 86) && mbar_wait_fast(vfull + v + 1, (uint32_t)(gt >> 1) & 1u, 86))) break;
+                    const unsigned long long lost = lost_sh[gt & 7];
                     const unsigned long long m0 = tree_tile_mask(t.see[0], pos, t.ctx) & ~lost, m1 = tree_tile_mask(t.see[1], pos, t.ctx) & ~lost;
                     for (int j = warp; j < TA_TILE; j += 4) {
                         if (((m0 & m1) >> j) & 1) continue;
