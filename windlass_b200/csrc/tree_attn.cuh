@@ -393,35 +393,36 @@ __device__ __forceinline__ unsigned long long tree_tile_mask(unsigned long long 
     const int first = pos0 - ctx;  // the tile's first key as a node number
     return first >= 64 ? 0ull : first >= 0 ? see >> first : (see << -first) | ((1ull << -first) - 1);
 }
-// This lane's box of a run of key tiles (a warp holds the nbox boxes of a tile): its page, loaded a tile ahead,
-// and its first row there; a tile on is `hop` pages and `rest` rows on.
+// This lane's box of every STEP-th tile of a run of key tiles (a warp holds the nbox boxes of a tile): its page,
+// loaded a step ahead, and its first row there; a step on is `hop` pages and `rest` rows on.
+template <int STEP = 1>
 struct TreePages {
     const int* table;
     int nbox, page_size, n_pages, end, hop, rest;
     int pos, at, off, page;
     bool mine;
-    __device__ void start(const TreeParams& p, const TreeItem& t) {
+    __device__ void start(const TreeParams& p, const TreeItem& t, int first = 0) {
         const int lane = threadIdx.x & 31, R = p.box_rows;
         table = p.table + (long long)t.b * p.table_stride;
         nbox = TA_TILE / R;
         page_size = p.page_size;
         n_pages = p.n_pages;
         end = t.ctx + t.n;
-        hop = TA_TILE / page_size;
-        rest = TA_TILE % page_size;
-        pos = t.tile0 * TA_TILE + lane * R;
+        hop = STEP * TA_TILE / page_size;
+        rest = STEP * TA_TILE % page_size;
+        pos = (t.tile0 + first) * TA_TILE + lane * R;
         at = pos / page_size;
         off = pos - at * page_size;
         mine = lane < nbox && pos < end;
         page = mine ? __ldg(table + at) : 0;
     }
     // First slot of this lane's box of the current tile, behind the pool (read as zeros) past the request's rows
-    // or for a page outside the pool (the error word, and `lost` then holds the tile's keys there), then a tile on.
+    // or for a page outside the pool (the error word, and `lost` then holds the tile's keys there), then a step on.
     __device__ int next(bool more, unsigned long long& lost) {
         const bool bad = mine && (page < 0 || page >= n_pages);
         if (bad) set_error(ERRC_BOUNDS, 46);
         const int slot = mine && !bad ? page * page_size + off : n_pages * page_size;
-        pos += TA_TILE;
+        pos += STEP * TA_TILE;
         at += hop;
         off += rest;
         if (off >= page_size) {
@@ -583,7 +584,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                     if (!more) break;
                     ++e;
                 }
-                TreePages pages;
+                TreePages<> pages;
                 pages.start(p, t);
                 const int nbox = pages.nbox;
                 const unsigned long long see = tree_mask_of(p, t.r0, t.n, t.node);

@@ -270,8 +270,9 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                 if (!ok) break;
                 ++use;
             }
-            TreePages pages;
-            if (more) pages.start(p, t);
+            const int own = (gt & 1) == which ? 0 : 1;  // this loader's first tile
+            TreePages<2> pages;
+            if (more) pages.start(p, t, own);
             if (which == 0) {
                 if (k >= 2 && !(ok = mbar_wait_fast(ifree + (k & 1), (uint32_t)((k >> 1) - 1) & 1u, 72))) break;
                 TpItem d{};
@@ -293,12 +294,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                 __syncwarp();
             }
             if (!more) break;
-            for (int i = 0; i < t.tiles; ++i, ++gt) {
+            for (int i = own; i < t.tiles; i += 2) {
                 unsigned long long lost;
-                const int slot = pages.next(i + 1 < t.tiles, lost);
-                if ((gt & 1) != which) continue;
+                const int slot = pages.next(i + 2 < t.tiles, lost);
                 if (lane < 8) slots[lane] = slot;
-                if (lane == 0) lost_sh[gt & 7] = lost;
+                if (lane == 0) lost_sh[(gt + i) & 7] = lost;
                 __syncwarp();
                 if (score) {
                     if (!(ok = acquire(0))) break;
@@ -315,6 +315,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                 }
                 ++use;
             }
+            gt += t.tiles;
         }
         if (!ok && use > 0)  // copies in flight must land before the CTA leaves
             for (int j = 0; j < steps; ++j) mbar_wait_fast(full + j, (uint32_t)(use - 1) & 1u, 73);
