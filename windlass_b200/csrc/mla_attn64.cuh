@@ -89,6 +89,12 @@ __device__ __forceinline__ void tma_load2d(uint32_t dst, const CUtensorMap* tm, 
         "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(smem_u32(bar))
         : "memory");
 }
+// The same from three dimensions.
+__device__ __forceinline__ void tma_load3d(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
 
 __global__ void __launch_bounds__(PF_THREADS, 1)
     mla_attn64_kernel(AttnParams p, const __grid_constant__ PfParams pp) {

@@ -77,6 +77,7 @@ struct TreeMaps {
     CUtensorMap q;     // {576, 64 n_nodes}, box {64, 64}
     CUtensorMap ckv;   // {512, slots}, box {64, box_rows}
     CUtensorMap krot;  // {64, slots}, box {64, box_rows}
+    CUtensorMap wide;  // tiles inside a page: the latent rows as {64, slots, 8 column chunks}, box {64, 64, 4}
     CUtensorMap part;  // the partials {512, 64 parts} fp32, box {32, 16}
     CUtensorMap out;   // ctx {512, 64 n_nodes}, box of 128 bytes x 16 rows
 };
@@ -453,10 +454,14 @@ __device__ __forceinline__ void tree_boxes(const TreeMaps& tm, uint32_t dst, int
     int y[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) y[j] = rows[j];
+    if constexpr (NB == 1) {  // a tile inside a page: its four column chunks at once (1 node x 1K 14.2 -> 13.7 us; pairs 1 % slower)
+        tma_load3d(dst + 4 * half * CHUNK, &tm.wide, 0, y[0], 4 * half, bar);
+    } else {
 #pragma unroll(NB <= 2 ? 4 : 1)
-    for (int c = 4 * half; c < 4 * half + 4; ++c) {
+        for (int c = 4 * half; c < 4 * half + 4; ++c) {
 #pragma unroll
-        for (int j = 0; j < NB; ++j) tma_load2d(dst + c * CHUNK + j * BOX, &tm.ckv, c * 64, y[j], bar);
+            for (int j = 0; j < NB; ++j) tma_load2d(dst + c * CHUNK + j * BOX, &tm.ckv, c * 64, y[j], bar);
+        }
     }
     if (half == 0) {
 #pragma unroll

@@ -241,6 +241,25 @@ int encode_bf16_2d(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t o
     return WL_OK;
 }
 
+// Latent rows [rows, 512] bf16 as {64, rows, 8}: a box takes four blocks of 64 columns of 64 rows, block after
+// block (128 bytes of a row are one swizzled line, as in the two-dimensional boxes).
+int encode_latent_chunks(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t row_elems) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return WL_ERR_CUDA;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)rows, 8};
+    const cuuint64_t strides[2] = {(cuuint64_t)row_elems * 2, 128};
+    const cuuint32_t box[3] = {64, 64, 4};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        std::fprintf(stderr, "wl_attn: cuTensorMapEncodeTiled (latent rows) failed (%d)\n", (int)r);
+        return WL_ERR_CUDA;
+    }
+    return WL_OK;
+}
+
 // One of the tensor-core weight products (gemv_tc.cuh), programmatic launch;
 // the query projection as 4-CTA clusters along K.
 template <int MODE>
@@ -1457,6 +1476,8 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (!p.sel) {
         if (int e = encode_bf16_2d(&tm.ckv, kv.latent.c_kv, wl::AT_DV, slots, kv.latent.c_kv_row_stride, 64, p.box_rows)) return e;
+        if (!pairs && p.box_rows == wl::TA_TILE)
+            if (int e = encode_latent_chunks(&tm.wide, kv.latent.c_kv, slots, kv.latent.c_kv_row_stride)) return e;
         if (int e = encode_bf16_2d(&tm.krot, kv.latent.k_rot, wl::AT_D - wl::AT_DV, slots, kv.latent.k_rot_row_stride, 64, p.box_rows))
             return e;
     }
