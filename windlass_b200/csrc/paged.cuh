@@ -6,8 +6,8 @@
 // dependent loads and launches. Each operator is one launch (a plan with many
 // tokens two), its sums run in shared memory, and every result is a fixed
 // function of the inputs (no atomics decide an order). Measured: a plan of 64
-// requests with 795 tokens 4.7 us, of 24 prompts with 73K tokens 8.0 us; a
-// commit of 8 requests in 78 layers 3.6 us, of 64 in one owner layer 5.2 us.
+// requests with 795 tokens 4.9 us, of 24 prompts with 73K tokens 8.2 us; a
+// commit of 8 requests in 78 layers 3.7 us, of 64 in one owner layer 5.3 us.
 #pragma once
 #include "ptx.cuh"
 

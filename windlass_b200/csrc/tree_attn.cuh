@@ -36,7 +36,7 @@
 // and the query in lanes 16-31.
 // Bound: with one node a request by HBM (148 requests x 8K keys 229 us, 6.1 TB/s; 6.7 in the
 // middle, 1.63 us a tile), with more nodes by the MMAs, which with M = 64 run at half rate
-// (2,176 cycles a tile), and in small calls by latency: 1 node x 1K keys 13.1 us, of
+// (2,176 cycles a tile), and in small calls by latency: 1 node x 1K keys 13.5 us, of
 // which the schedule 1.1, query and first tile 2.5, output 3, join 2.5.
 // Roundings: scores, maxima, sums and O are fp32; only P enters P.V in bf16 (the
 // tensor core's operand type: the cache is bf16); l sums P before that rounding.

@@ -19,10 +19,10 @@
 // cycles, where tree_attn_kernel's two SMs take 2 x 2,176 for the same. Each key
 // row is read by both CTAs (from L2 once more), 64 bytes a cycle and SM.
 // Bound: shared-memory bandwidth. A score SM writes 72 KB of keys, reads them for the MMAs and
-// writes and sends 16 KB of P, a value SM likewise: 1,410 cycles at 128 bytes; 1,450 to
-// 1,620 measured, at clocks that the power cap brings down to 1.6 to 1.75 GHz.
-// 394 nodes of 16 requests x 32K keys 1,150 us cold, 1,240 to 1,310 warm (1.08 to 1.22 PFLOP/s,
-// of 1.38 sustained); 92 nodes of 8 x 16K 158 to 166 us.
+// writes and sends 16 KB of P, a value SM likewise: 1,410 cycles at 128 bytes; 1,434
+// (1 request x 64 nodes x 30K) and 1,484 (9 x 16 x 16K) measured.
+// 394 nodes of 16 requests x 32K keys 1,080 us, 1,110 to 1,220 once the power cap brings the
+// clock down to 1.6 to 1.75 GHz (1.16 to 1.31 PFLOP/s); 92 nodes of 8 x 16K 148 to 154 us.
 // Two nodes share V in one MMA: a drafted row that not both see, and that holds
 // a NaN or an infinity, would reach the other through 0 x NaN. In tiles with
 // drafted rows the value CTA therefore clears rows that neither sees and the

@@ -1464,7 +1464,7 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     // row's request filled its table row. One at a time / pairs, us:
     //   by keys      20 nodes x 4K 28 / 37; 16 x 8K 36 / 45; 64 x 1K 30 / 36; 45 x 4K 39 / 42; 57 x 3K 38 / 41;
     //                64 x 4K 59 / 56; 32 x 8K 56 / 51; 35 x 8K 58 / 53; 12 x 60K 120 / 115; 16 x 30K 84 / 72;
-    //                92 x 16K 190 / 160; 394 x 32K 1625 / 1200
+    //                92 x 16K 190 / 150; 394 x 32K 1625 / 1080
     //   by tree      46 of 16 requests x 8K 67 / 67; 40 of 17 x 13K 94 / 99; 90 of 15 x 2.6K 65 / 55; 11 of 4 x 30K 52 / 59
     const int64_t room = (int64_t)kv.max_pages * kv.page_size, most = room < cfg->T_max ? room : cfg->T_max;
     const bool pairs = !p.sel && io->n_nodes >= 12 && (int64_t)io->n_nodes >= 6 * (int64_t)io->batch &&
