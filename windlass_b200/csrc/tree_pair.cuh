@@ -15,9 +15,9 @@
 //   value CTA  O += P V: 8 MMAs M = 128, N = 256: 1,024 cycles. Four warps rescale
 //              O when a factor is not 1 (rare: the maximum moves only by more than
 //              2^8), and write O / l at the end of an item.
-// So both tensor cores work all the time, on 64 keys of two nodes in about 1,152
-// cycles, where tree_attn_kernel's two SMs take 2 x 2,176 for the same. Each key
-// row is read by both CTAs (from L2 once more), 64 bytes a cycle and SM.
+// So both SMs work on the same 64 keys of two nodes, in 1,434 to 1,484 cycles, where
+// two SMs of tree_attn_kernel take 2,176 for one node each. Each key row is read by
+// both CTAs (from L2 once more), 50 bytes a cycle and SM.
 // Bound: shared-memory bandwidth. A score SM writes 72 KB of keys, reads them for the MMAs and
 // writes and sends 16 KB of P, a value SM likewise: 1,410 cycles at 128 bytes; 1,434
 // (1 request x 64 nodes x 30K) and 1,484 (9 x 16 x 16K) measured.

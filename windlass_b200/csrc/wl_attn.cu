@@ -1459,16 +1459,16 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     wl::TreeMaps tm{};
     if (int e = encode_q_map(&tm.q, io->q_abs, io->n_nodes)) return e;
     // Two nodes of a request at a time, by CTA pairs, when there is enough to do; one at a time for small trees (a
-    // lone or last odd node leaves half of a pair's rows empty), for few keys (the pair's start and end take 8 us
+    // lone or last odd node leaves half of a pair's rows empty), for few keys (the pair's start and end take 5 us
     // longer) and for lists (a list per node). The lengths are on the device, so the keys are counted as if every
     // row's request filled its table row. One at a time / pairs, us:
-    //   by keys      20 nodes x 4K 28 / 37; 16 x 8K 36 / 45; 64 x 1K 30 / 36; 45 x 4K 39 / 42; 57 x 3K 38 / 41;
-    //                64 x 4K 59 / 56; 32 x 8K 56 / 51; 35 x 8K 58 / 53; 12 x 60K 120 / 115; 16 x 30K 84 / 72;
+    //   by keys      64 nodes x 1K 31 / 36; 40 x 2K 31 / 33; 16 x 8K 37 / 38; 64 x 2.5K 48 / 47; 47 x 4K 44 / 45;
+    //                40 x 5K 54 / 48; 21 x 10K 45 / 42; 16 x 14K 52 / 47; 32 x 8K 60 / 52; 12 x 60K 120 / 115;
     //                92 x 16K 190 / 150; 394 x 32K 1625 / 1080
     //   by tree      46 of 16 requests x 8K 67 / 67; 40 of 17 x 13K 94 / 99; 90 of 15 x 2.6K 65 / 55; 11 of 4 x 30K 52 / 59
     const int64_t room = (int64_t)kv.max_pages * kv.page_size, most = room < cfg->T_max ? room : cfg->T_max;
     const bool pairs = !p.sel && io->n_nodes >= 12 && (int64_t)io->n_nodes >= 6 * (int64_t)io->batch &&
-                       (int64_t)io->n_nodes * most >= 240 * 1024;
+                       (int64_t)io->n_nodes * most >= 160 * 1024;
     const uint32_t out_rows = pairs ? 32 : 16;  // a warp's rows
     if (int e = encode_out_map(&tm.part, p.o_part, parts, false, out_rows)) return e;
     if (int e = encode_out_map(&tm.out, io->ctx, io->n_nodes, p.ctx_bf16, out_rows)) return e;
