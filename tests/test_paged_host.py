@@ -1,6 +1,8 @@
 """Refusals of the paged-cache and drafted-tree entry points (argument checks run before
 any launch, so no GPU is needed), and the restatement's own consistency."""
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
@@ -155,6 +157,35 @@ def test_python_checks_run_before_any_launch():
             P.PagedKV(**f)
     with pytest.raises(ValueError):
         P.LayerCaches([])
+
+
+def layout(name, **known):
+    """The uint32_t constants of a shared-memory layout in tree_pair.cuh."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "windlass_b200", "csrc", "tree_pair.cuh")
+    with open(path) as f:
+        src = f.read()
+    vals = {k: int(v) for k, v in re.findall(r"constexpr int (TP_\w+) = (\d+);", src)}
+    vals.update(known)
+    for k, v in re.findall(r"static constexpr \w+ (\w+) = (.*?);", src[src.index("struct " + name):]):
+        if "idesc" not in v:
+            for part in [x.split("=") for x in (k + "=" + v).split(", ")]:
+                vals[part[0].strip()] = eval(part[1], {}, vals)
+    return vals, src
+
+
+def test_no_copy_of_the_other_cta_lands_on_the_schedule():
+    """The score CTA sends P, rescale factors and 1 / l into the value CTA's shared memory as soon as it has them: the value
+    CTA's schedule, which nothing holds them back for, lies elsewhere."""
+    v, src = layout("TpLayout", TA_TILE=64)
+    assert re.search(r"cost = reinterpret_cast<TreeCost\*>\(smem \+ L::OFF_SCHED\)", src)
+    assert re.search(r"tab = reinterpret_cast<int2\*>\(many \? smem : smem \+ L::OFF_SCHED \+ sizeof\(TreeCost\)\)", src)
+    cost = 4 * 3 * 64 * 4 + 32 * 8  # four sums for three thirds of the requests and 64 choices; (nodes, tiles) of 32 requests
+    sched = (v["OFF_SCHED"], v["OFF_SCHED"] + cost)
+    many = (0, 16384 * 8)  # the table of more requests
+    for first, size in ((v["OFF_P"], v["TP_P"] * v["P"]), (v["OFF_ALPHA"], v["TP_P"] * 512), (v["OFF_FIN"], 512),
+                        (v["OFF_BAR"], 8 * v["N_BARS"])):
+        for a, b in (sched, many):
+            assert b <= first or first + size <= a
 
 
 # ---- the restatement -------------------------------------------------------------------------

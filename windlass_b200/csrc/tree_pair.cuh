@@ -54,6 +54,10 @@ struct TpLayout {
     static constexpr uint32_t P = 128 * 128;                  // 128 rows x 64 keys bf16
     static constexpr uint32_t OFF_P = TP_HALVES * HALF;       // value CTA
     static constexpr uint32_t OFF_PS = TP_UNITS * UNIT;       // score CTA: P on its way
+    // Both: the schedule's sums and table. The score CTA's first copies of P may reach a value CTA that is still at its
+    // schedule (nothing waits for it before), so the scratch is behind P there; in the score CTA it is the place of
+    // the fourth tile of P, which only that CTA writes, after its schedule.
+    static constexpr uint32_t OFF_SCHED = OFF_P + TP_P * P;
     static constexpr uint32_t OFF_ALPHA = OFF_PS + TP_P * P;  // both: rescale factors [TP_P][128]
     static constexpr uint32_t OFF_FIN = OFF_ALPHA + TP_P * 512;  // value CTA: 1 / l of the item's rows [128]
     static constexpr uint32_t OFF_MAX = OFF_FIN + 512;        // score CTA: rows' maxima after even and odd tiles [2][128]
@@ -68,7 +72,8 @@ struct TpLayout {
     static constexpr uint32_t IDESC_PV = idesc_bf16(128, 256, 0, 1);
 };
 static_assert(TpLayout::BYTES <= 232448, "one CTA per SM");
-static_assert(TP_P == 4 && TpLayout::OFF_P + TP_P * TpLayout::P <= TpLayout::OFF_ALPHA, "value CTA's layout");
+static_assert(TP_P == 4 && TpLayout::OFF_SCHED + sizeof(TreeCost) + 32 * sizeof(int2) <= TpLayout::OFF_ALPHA, "value CTA's layout");
+static_assert(TpLayout::OFF_SCHED >= TpLayout::OFF_PS, "score CTA's layout: no key tile over the schedule");
 
 struct TpItem {  // what the roles of a CTA need of an item
     int rows, row0;        // nodes (1 or 2; 0: no more), first row
@@ -196,9 +201,9 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
     pdl_trigger();
-    TreeCost* cost = reinterpret_cast<TreeCost*>(smem + L::OFF_P);
+    TreeCost* cost = reinterpret_cast<TreeCost*>(smem + L::OFF_SCHED);
     const bool many = p.batch > 32;
-    int2* tab = reinterpret_cast<int2*>(many ? smem : smem + L::OFF_P + sizeof(TreeCost));
+    int2* tab = reinterpret_cast<int2*>(many ? smem : smem + L::OFF_SCHED + sizeof(TreeCost));
     TreeWalk<false, 2> walk;
     if (many) {
         if (tid == 0) *longest_sh = 0;
