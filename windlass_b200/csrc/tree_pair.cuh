@@ -490,6 +490,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
             mbar_arrive(ldone);
             if (!(ok = mbar_wait_fast(ldone, (uint32_t)k & 1u, 91))) break;  // all of its threads are this far
         }
+        // The last tiles of P: the value CTA's word that their places are free must be here before this CTA leaves.
+        for (int pb = s; ok && pb < TP_P && pb < gt; pb += 2) ok = mbar_wait_cluster(pfree + pb, (uint32_t)((gt - 1 - pb) >> 2) & 1u, 80);
     } else if (warp == TP_MMA_WARP) {
         // ---------------- value CTA: P V ----------------
         int gt = 0;
