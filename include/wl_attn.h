@@ -408,15 +408,18 @@ int wl_cache_append(const wl_attn_cfg* cfg, const wl_cache_append_io* io, void* 
  * block_table[b][p / page_size] * page_size + p % page_size. The pool is a
  * wl_latent_cache / wl_index_cache of one sequence (the seq strides are not
  * used). Speculative decoding writes every drafted token of a request behind
- * its context (drafted node i at position ctx_len + i), scores all of them in
- * one attention call, then keeps the accepted path:
+ * its context (drafted node i in the row of position ctx_len + i), scores all
+ * of them in one attention call, then keeps the accepted path:
  *   wl_page_plan -> wl_cache_append_paged (per layer) -> wl_mla_tree_attn (per
  *   layer) -> wl_tree_commit.
  * No counterpart in the reference: it decodes one sequence, one token at a
  * time, into caches of max_seq rows (glm_loader.cuh:282-307). All lengths live
  * on the device, so a captured graph serves changing requests. A request may
  * have 0 to 64 drafted nodes; node 0 is the token chosen last (its cache row
- * is not committed yet), later nodes hang from earlier ones. */
+ * is not committed yet), later nodes hang from earlier ones. The rotation of a
+ * node's query and keys is by its place on its branch, ctx_len + depth: what
+ * its row keeps when the path that it stands on is committed. wl_page_plan
+ * gives these positions when it is given the trees. */
 enum { WL_TREE_MAX = 64 };
 enum { WL_F32 = 0, WL_BF16 = 1 };
 
@@ -443,7 +446,13 @@ typedef struct wl_paged_kv {
  * and no tokens. Tokens are laid out request after request: token i of
  * request b is row cu_new[b] + i. Rows behind the last token (a padded batch)
  * get -1. More tokens than n_tokens set the error word; the rows that fit are
- * written. n_held_out / n_free_out may be n_held / n_free (updated in place). */
+ * written. n_held_out / n_free_out may be n_held / n_free (updated in place).
+ * slot goes by the token's number in its request, pos is its position in the
+ * text, by which its query and keys are rotated: ctx_len + i, or, with the trees
+ * that wl_mla_tree_attn gets (parent or tree_mask, rows cu_new[b] + i), ctx_len +
+ * the number of its ancestors (of the other nodes that its mask names), so that
+ * siblings share a position. A request of more than WL_TREE_MAX tokens is a
+ * prompt: its rows stay ctx_len + i. */
 typedef struct wl_page_plan_io {
     int32_t batch;
     int32_t n_tokens;              /* rows of slot / pos / seq                       */
@@ -464,6 +473,8 @@ typedef struct wl_page_plan_io {
     int32_t* slot;                 /* out, device [n_tokens] (may be NULL if n_tokens is 0) */
     int32_t* pos;                  /* out, device [n_tokens]                         */
     int32_t* seq;                  /* out, device [n_tokens]                         */
+    const int32_t*  parent;        /* device [n_tokens] or NULL: the trees, by parents */
+    const uint64_t* tree_mask;     /* device [n_tokens] or NULL: or by masks         */
 } wl_page_plan_io;
 
 int wl_page_plan(const wl_page_plan_io* io, void* stream);

@@ -1,0 +1,157 @@
+"""Positions of drafted trees in a plan, and whole steps with rotated keys, on the GPU. Everything here is
+compared bit for bit: whole numbers, and rows that the plain append writes at the same positions."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_ref as R
+from test_gpu_paged import SCALE, T_MAX, bad_word, clean_device_error, cpu, i32  # noqa: F401
+from windlass_b200 import attn as A
+from windlass_b200 import paged as P
+
+pytestmark = pytest.mark.gpu
+
+
+def signed(masks):
+    return torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks], dtype=torch.int64, device="cuda")
+
+
+def random_trees(rng, sizes, back=4):
+    return np.concatenate([[-1] + [rng.integers(max(0, j - back), j) for j in range(1, n)] if n else [] for n in sizes]).astype(np.int32)
+
+
+def plan_of(ctx, new, page, n_tokens, **kw):
+    """A plan for requests that hold what their contexts need, with pages enough."""
+    ctx, new = np.asarray(ctx), np.asarray(new)
+    held, most = -(-ctx // page), -(-(ctx + new) // page)
+    n_pages = int(most.sum()) + 1
+    table, at = np.zeros((len(ctx), max(int(most.max()), 1)), np.int32), 0
+    for b, h in enumerate(held):
+        table[b, :h] = np.arange(at, at + h)
+        at += h
+    free = np.zeros(n_pages, np.int32)
+    free[:n_pages - at] = np.arange(at, n_pages)
+    return P.page_plan(i32(ctx), i32(new), i32(table), i32(held), i32(free), i32([n_pages - at]), page, n_tokens, **kw)
+
+
+# one launch and two, padded and not
+@pytest.mark.parametrize("B,most,spare", [(1, 1, 0), (1, 64, 0), (9, 16, 5), (70, 64, 0), (1100, 3, 2), (40, 64, 1000)])
+def test_positions_of_trees_count_ancestors(B, most, spare):
+    rng = np.random.default_rng(B + most)
+    ctx, new = rng.integers(0, 500, B), rng.integers(0, most + 1, B)
+    new[0] = most
+    total = int(new.sum())
+    parent = random_trees(rng, new)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    masks = R.tree_masks(parent, cu)
+    seq = np.repeat(np.arange(B), new)
+    want = ctx[seq] + [bin(m).count("1") - 1 for m in masks]
+    line = plan_of(ctx, new, 16, total + spare)
+    for kw in (dict(parent=i32(np.pad(parent, (0, spare)))), dict(mask=signed(masks + [0] * spare))):
+        got = plan_of(ctx, new, 16, total + spare, **kw)
+        assert np.array_equal(cpu(got["pos"]), np.pad(want, (0, spare), constant_values=-1))
+        for k in ("slot", "seq", "cu", "short", "n_held", "n_free"):
+            assert torch.equal(got[k], line[k]), k
+    assert np.array_equal(cpu(line["pos"])[:total], ctx[seq] + np.arange(total) - cu[seq])
+
+
+def test_positions_of_prompts_roots_and_bad_parents():
+    parent = i32([-1, 0, 0, -1, 3, 1] + [0] * 65)  # two roots in the first request, a prompt of 65 tokens behind it
+    got = plan_of([10, 7], [6, 65], 8, 71, parent=parent)
+    assert cpu(got["pos"])[:6].tolist() == [10, 11, 11, 10, 11, 12]
+    assert cpu(got["pos"])[6:].tolist() == list(range(7, 72))
+    got = plan_of([3], [4], 8, 4, parent=i32([-1, 1, 3, 2]))  # itself, and a later node
+    bad_word()
+    assert cpu(got["pos"]).tolist() == [3, 3, 3, 4]
+    got = plan_of([3], [3], 8, 3, mask=signed([(1 << 64) - 1, 0, 0b1000]))  # later nodes and itself, none, no node of the request
+    assert cpu(got["pos"]).tolist() == [5, 3, 3]
+
+
+@pytest.mark.parametrize("by", ["parent", "mask"])
+def test_branched_steps_leave_what_appending_the_accepted_tokens_leaves(by):
+    """Drafted trees with a real RoPE table, three steps, captured once: after every commit the pools of latent rows, index
+    keys and scales hold, bit for bit, what appending the accepted tokens one by one at their positions leaves, and the
+    attention of every node saw the keys of its branch, rotated by their places on it."""
+    page, B, L, N = 8, 2, 2, 12
+    rng = np.random.default_rng(31)
+    cfg = A.glm52_cfg(T_MAX)
+    angle = np.arange(80)[:, None] / 10000 ** (np.arange(32) / 32)
+    cos_t, sin_t = (torch.tensor(f(angle), dtype=torch.float32, device="cuda") for f in (np.cos, np.sin))
+    pool = [torch.zeros(24 * page, 576, device="cuda", dtype=torch.bfloat16) for _ in range(L)]
+    ikeys = A.IndexKeys(torch.zeros(24 * page, 128, dtype=torch.uint8, device="cuda"), torch.zeros(24 * page, device="cuda"))
+    table, held, free = i32(np.zeros((B, 8))), i32([0] * B), i32(rng.permutation(24))
+    n_free, ctx_len, n_new = i32([24]), i32([0] * B), i32([0] * B)
+    kvs = [P.PagedKV.packed(x, page, table) for x in pool]
+    caches = P.LayerCaches(kvs, [ikeys, None])
+    g = torch.Generator(device="cuda").manual_seed(3)
+    norm = torch.rand(512, generator=g, device="cuda").to(torch.bfloat16)
+    kw_, kb_ = (torch.rand(128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    raw, kraw = torch.zeros(L, N, 576, device="cuda"), torch.zeros(N, 128, device="cuda")
+    q = torch.randn(N, 64, 576, generator=g, device="cuda").to(torch.bfloat16)
+    parent, draft, target = i32([0] * N), i32([0] * N), i32([0] * N)
+    mask = torch.zeros(N, dtype=torch.int64, device="cuda")
+    trees = dict(parent=parent) if by == "parent" else dict(mask=mask)
+
+    def step():
+        plan = P.page_plan(ctx_len, n_new, table, held, free, n_free, page, N, in_place=True, **trees)
+        cos, sin = cos_t[plan["pos"]], sin_t[plan["pos"]]
+        outs = []
+        for i in range(L):
+            P.cache_append_paged(cfg, plan["slot"], cos, sin, kv=kvs[i], kv_raw=raw[i], kv_norm_w=norm,
+                                 **(dict(keys=ikeys, k_raw=kraw, k_norm_w=kw_, k_norm_b=kb_) if i == 0 else {}))
+            outs.append(P.mla_tree_attn(cfg, kvs[i], q, ctx_len, plan["cu"], **trees))
+        return plan, outs, P.tree_commit(caches, ctx_len, plan["cu"], parent, draft, target)
+
+    step()  # nothing to do: loads the kernels
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan, outs, done = step()
+
+    # the plain sequences: one contiguous cache per request and layer, appended token by token
+    flat = [[torch.zeros(1, 64, 576, device="cuda", dtype=torch.bfloat16) for _ in range(B)] for _ in range(L)]
+    fkeys = [A.IndexKeys(torch.zeros(1, 64, 128, dtype=torch.uint8, device="cuda"), torch.zeros(1, 64, device="cuda")) for _ in range(B)]
+
+    def append(b, row, pos):
+        at = i32([pos])
+        for i in range(L):
+            A.cache_append(cfg, at, cos_t[pos:pos + 1], sin_t[pos:pos + 1], kv=A.LatentKV.packed(flat[i][b]), kv_raw=raw[i, row:row + 1],
+                           kv_norm_w=norm, **(dict(keys=fkeys[b], k_raw=kraw[row:row + 1], k_norm_w=kw_, k_norm_b=kb_) if i == 0 else {}))
+
+    jumped = 0
+    for sizes in ([6, 6], [7, 5], [9, 3], [0, 12]):
+        n_new.copy_(i32(sizes))
+        par = np.concatenate([random_trees(rng, sizes), np.zeros(N - sum(sizes))]).astype(np.int32)
+        dr, tg = rng.integers(0, 2, N), rng.integers(0, 2, N)
+        cu = np.concatenate([[0], np.cumsum(sizes)])
+        masks = R.tree_masks(par, cu)
+        parent.copy_(i32(par)), draft.copy_(i32(dr)), target.copy_(i32(tg)), mask.copy_(signed(masks + [0] * (N - len(masks))))
+        raw.copy_(torch.randn(L, N, 576, generator=g, device="cuda")), kraw.copy_(torch.randn(N, 128, generator=g, device="cuda"))
+        ctx = cpu(ctx_len).tolist()
+        graph.replay()
+        torch.cuda.synchronize()
+        for b in range(B):
+            for j in range(sizes[b]):  # every node alone on its branch
+                r = cu[b] + j
+                for d, a in enumerate([a for a in range(j + 1) if masks[r] >> a & 1]):
+                    append(b, cu[b] + a, ctx[b] + d)
+                depth = bin(masks[r]).count("1")
+                for i in range(L):
+                    rows = flat[i][b][0].float().cpu().numpy()
+                    ref, lse, spread = R.tree_attn(q[r:r + 1].float().cpu().numpy(), rows, [ctx[b] + depth - 1], [0, 1], [1],
+                                                   np.arange(8, dtype=np.int32)[None], 8, SCALE)
+                    # P in bf16, 2 DS of q and k of unit size below 4e-4 (k: at most 1 after the norm's weights below 1)
+                    assert np.all(np.abs(cpu(outs[i]["ctx"])[r:r + 1] - ref) <= (2.0 ** -8 + 4e-4) * spread)
+                    assert np.abs(cpu(outs[i]["lse"])[r:r + 1] - lse).max() < 4e-4
+            path, _ = R.tree_walk(par[cu[b]:cu[b + 1]], dr[cu[b]:cu[b + 1]], tg[cu[b]:cu[b + 1]])
+            jumped += path != list(range(len(path)))
+            for d, j in enumerate(path):
+                append(b, cu[b] + j, ctx[b] + d)
+            assert int(done["n_accept"][b]) == len(path)
+            pos = np.arange(ctx[b] + len(path))
+            slots = torch.from_numpy(cpu(table)[b][pos // page].astype(np.int64) * page + pos % page).cuda()
+            for i in range(L):
+                assert torch.equal(pool[i][slots], flat[i][b][0, :len(pos)])
+            assert torch.equal(ikeys.keys[slots], fkeys[b].keys[0, :len(pos)])
+            assert torch.equal(ikeys.scale[slots], fkeys[b].scale[0, :len(pos)])
+        ctx_len.copy_(done["ctx_len"])
+    assert jumped >= 2  # the paths left the line

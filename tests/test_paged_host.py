@@ -188,6 +188,19 @@ def test_no_copy_of_the_other_cta_lands_on_the_schedule():
             assert b <= first or first + size <= a
 
 
+def test_page_plan_takes_the_trees_in_one_form():
+    assert lib().wl_page_plan(C.byref(plan_io(parent=FAKE, tree_mask=FAKE)), None) == ARG
+    z = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="not both"):
+        P.page_plan(z, z, z.view(4, 1), z, z, z, 8, 4, parent=z, mask=z.long())
+    with pytest.raises(ValueError, match="parent must hold 4"):
+        P.page_plan(z, z, z.view(4, 1), z, z, z, 8, 4, parent=z[:3])
+    with pytest.raises(ValueError, match="int32"):
+        P.page_plan(z, z, z.view(4, 1), z, z, z, 8, 4, parent=z.long())
+    with pytest.raises(ValueError, match="int64"):
+        P.page_plan(z, z, z.view(4, 1), z, z, z, 8, 4, mask=z)
+
+
 # ---- the restatement -------------------------------------------------------------------------
 
 def test_restated_plan_gives_every_position_its_own_slot():

@@ -87,7 +87,7 @@ class PagePlanIO(C.Structure):
                 ("n_new", vp), ("block_table", vp), ("table_stride", i64), ("max_pages", i32),
                 ("n_held", vp), ("n_held_out", vp), ("free_list", vp), ("n_free", vp),
                 ("n_free_out", vp), ("cu_new", vp), ("short_out", vp), ("slot", vp), ("pos", vp),
-                ("seq", vp)]
+                ("seq", vp), ("parent", vp), ("tree_mask", vp)]
 
 
 class TreeAttnIO(C.Structure):

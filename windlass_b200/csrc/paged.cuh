@@ -33,6 +33,8 @@ struct PlanParams {
     int* slot;
     int* pos;
     int* seq;
+    const int* parent;               // with one of these, pos counts a drafted token's ancestors, not its predecessors
+    const unsigned long long* mask;
     int own_tokens;  // the plan kernel writes the token rows too
 };
 
@@ -90,11 +92,34 @@ __device__ __forceinline__ int page_slot(const int* row, int page_size, int n_pa
     return page * page_size + pos % page_size;
 }
 
-// One token row (shared by the plan kernel and plan_tokens_kernel).
-__device__ __forceinline__ void plan_token(const PlanParams& p, int i, int b, int first, int lack, int ctx) {
-    const int pos = ctx + (i - first);
+// Depth of node j of a request's tree (`parent` from its first row on): the number of its ancestors, which stand
+// before it. A parent that does not sets the error word and counts as none, as in the attention's masks.
+__device__ __forceinline__ int plan_depth(const int* parent, int j) {
+    int d = 0;
+    for (int at = j;;) {
+        const int up = __ldg(parent + at);
+        if (up < 0) return d;
+        if (up >= at) {
+            set_error(ERRC_BOUNDS, 45);
+            return d;
+        }
+        at = up;
+        ++d;
+    }
+}
+
+// One token row (shared by the plan kernel and plan_tokens_kernel): token i, of n that request b has from row
+// `first` on. Its cache row goes by its number in the request; its position in the text is that of a branch, so
+// siblings share one (a request of more than TREE_MAX tokens is a prompt: a line).
+__device__ __forceinline__ void plan_token(const PlanParams& p, int i, int b, int first, int n, int lack, int ctx) {
+    const int j = i - first, pos = ctx + j;
+    int deep = j;
+    if (n <= TREE_MAX) {
+        if (p.parent) deep = plan_depth(p.parent + first, j);
+        else if (p.mask) deep = __popcll(p.mask[i] & (n >= 64 ? ~0ull : (1ull << n) - 1) & ~(1ull << j));
+    }
     p.slot[i] = lack != 0 ? -1 : page_slot(p.table + (long long)b * p.table_stride, p.page_size, p.n_pages, pos, 41);
-    p.pos[i] = pos;
+    p.pos[i] = ctx + deep;
     p.seq[i] = b;
 }
 
@@ -181,7 +206,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanParams p) {
             const int t1 = min(sh_tok[nb], p.n_tokens);
             for (int i = sh_tok[0] + tid; i < t1; i += PLAN_THREADS) {
                 const int j = last_le(sh_tok, 0, nb, i);
-                plan_token(p, i, b0 + j, sh_tok[j], sh_lack[j], sh_ctx[j]);
+                plan_token(p, i, b0 + j, sh_tok[j], sh_tok[j + 1] - sh_tok[j], sh_lack[j], sh_ctx[j]);
             }
         }
         __syncthreads();  // shared arrays are reused
@@ -206,7 +231,7 @@ __global__ void __launch_bounds__(256) plan_tokens_kernel(PlanParams p) {
         return;
     }
     const int b = last_le(p.cu, 0, p.batch, i);
-    plan_token(p, i, b, p.cu[b], p.lack[b], p.ctx_len[b]);
+    plan_token(p, i, b, p.cu[b], p.cu[b + 1] - p.cu[b], p.lack[b], p.ctx_len[b]);
 }
 
 struct ReleaseParams {

@@ -1286,7 +1286,10 @@ int wl_page_plan(const wl_page_plan_io* io, void* stream) {
     if ((io->batch > 0 && (!io->ctx_len || !io->n_new || !io->n_held || !io->n_held_out || !io->short_out)) ||
         !io->free_list || !io->n_free || !io->n_free_out || !io->cu_new || (io->n_tokens > 0 && (!io->slot || !io->pos || !io->seq)))
         return WL_ERR_ARG;
+    if (io->parent && io->tree_mask) return WL_ERR_ARG;
     wl::PlanParams p{};
+    p.parent = io->parent;
+    p.mask = reinterpret_cast<const unsigned long long*>(io->tree_mask);
     p.batch = io->batch;
     p.n_tokens = io->n_tokens;
     p.page_size = io->page_size;

@@ -4,7 +4,8 @@ One pool of cache rows serves requests of different lengths: a page is ``page_si
 consecutive rows ("slots") and a request's block table lists its pages in position
 order. A step with drafted tokens is::
 
-    plan = page_plan(ctx_len, n_new, table, n_held, free_list, n_free, page_size, n_tokens)
+    plan = page_plan(ctx_len, n_new, table, n_held, free_list, n_free, page_size, n_tokens, parent=parent)
+    cos, sin = cos_table[plan["pos"]], sin_table[plan["pos"]]                   # of the queries too
     cache_append_paged(cfg, plan["slot"], cos, sin, kv=kv, kv_raw=..., ...)     # each layer
     out = mla_tree_attn(cfg, kv, q_abs, ctx_len, plan["cu"], parent=parent)     # each layer
     done = tree_commit(layers, ctx_len, plan["cu"], parent, draft, target)
@@ -54,6 +55,17 @@ def _table(t: torch.Tensor, batch: int, dev: torch.device) -> tuple[int, int, in
     if rows < batch or (width > 1 and col != 1) or (batch > 1 and row < width):
         raise ValueError(f"block_table must have {batch} rows of consecutive entries")
     return t.data_ptr(), row if batch > 1 else max(width, 1), width
+
+
+def _trees(parent: torch.Tensor | None, mask: torch.Tensor | None, n: int, dev: torch.device) -> tuple:
+    """Addresses of the trees of ``n`` rows: parents (int32) or masks (int64), the other None."""
+    if parent is not None and mask is not None:
+        raise ValueError("give parent or mask, not both")
+    if mask is None:
+        return None if parent is None else _i32(parent, "parent", dev, n), None
+    if mask.dtype != torch.int64 or mask.device != dev or not mask.is_contiguous() or mask.numel() < n:
+        raise ValueError(f"mask must be a contiguous int64 tensor of {n} elements on {dev}")
+    return None, mask.data_ptr()
 
 
 def _call(dev: torch.device, fn, *args) -> int:
@@ -110,13 +122,19 @@ class PagedKV:
 
 def page_plan(ctx_len: torch.Tensor, n_new: torch.Tensor, block_table: torch.Tensor, n_held: torch.Tensor,
               free_list: torch.Tensor, n_free: torch.Tensor, page_size: int, n_tokens: int, *,
-              in_place: bool = False) -> dict:
+              in_place: bool = False, parent: torch.Tensor | None = None, mask: torch.Tensor | None = None) -> dict:
     """Pages and slots for ``n_new[b]`` tokens behind ``ctx_len[b]`` cached ones
     (``wl_page_plan``). New pages come from the top of the stack ``free_list[:n_free]`` in
     request order and are written into ``block_table``. Returns slot, pos, seq
     [n_tokens] (rows behind the last token: -1), cu [batch + 1], short [batch] (pages a
     request lacks; such a request gets none, and slots and table entries of -1), n_held [batch] and
-    n_free [1] after the call: new tensors, or the given ones with ``in_place``."""
+    n_free [1] after the call: new tensors, or the given ones with ``in_place``.
+
+    ``pos`` is what a token's query and keys are rotated by: ``ctx_len`` + its number in the
+    request, or, with the trees that ``mla_tree_attn`` gets (``parent`` or ``mask``, at least
+    [n_tokens]), ``ctx_len`` + the number of its ancestors (the other nodes of its mask), so
+    that siblings share a position. Slots are one a token either way. A request of more than 64 tokens is a
+    prompt: its positions run on."""
     dev = ctx_len.device
     B, T = ctx_len.numel(), int(n_tokens)
     c, n, held, nf = (_i32(ctx_len, "ctx_len", dev), _i32(n_new, "n_new", dev, B), _i32(n_held, "n_held", dev, B),
@@ -125,6 +143,7 @@ def page_plan(ctx_len: torch.Tensor, n_new: torch.Tensor, block_table: torch.Ten
     free = _i32(free_list, "free_list", dev)
     if T < 0:
         raise ValueError("n_tokens must not be negative")
+    par, m = _trees(parent, mask, T, dev)
     # one allocation: slot, pos, seq [T], cu [B + 1], short [B] and, unless in place, n_held [B] and n_free [1]
     sizes = [T, T, T, B + 1, B] if in_place else [T, T, T, B + 1, B, B, 1]
     out = torch.empty(sum(sizes), dtype=_I32, device=dev)
@@ -132,7 +151,7 @@ def page_plan(ctx_len: torch.Tensor, n_new: torch.Tensor, block_table: torch.Ten
     short = o + 4 * (3 * T + B + 1)
     io = _lib.PagePlanIO(B, T, page_size, free_list.numel(), c, n, table, stride, width, held,
                          held if in_place else short + 4 * B, free, nf, nf if in_place else short + 8 * B, o + 12 * T,
-                         short, o, o + 4 * T, o + 8 * T)
+                         short, o, o + 4 * T, o + 8 * T, par, m)
     check(_call(dev, lib().wl_page_plan, C.byref(io)), "wl_page_plan")
     parts = torch.unsafe_split_with_sizes(out, sizes)  # (integers: no gradient to track, and `out` ends here)
     return dict(slot=parts[0], pos=parts[1], seq=parts[2], cu=parts[3], short=parts[4],
@@ -175,7 +194,7 @@ def mla_tree_attn(cfg: AttnCfg, kv: PagedKV, q_abs: torch.Tensor, ctx_len: torch
     """Absorbed-MLA attention of every request's drafted nodes (``wl_mla_tree_attn``).
 
     q_abs bf16 [n, 64, 576]; request b's rows are ``cu_nodes[b]:cu_nodes[b + 1]`` and its
-    node i sits at position ``ctx_len[b] + i``. A row sees the context and its
+    node i's cache row is that of position ``ctx_len[b] + i`` (``page_plan``'s slot; rotated by its ``pos``). A row sees the context and its
     ancestors by ``parent`` [n] (int32, index within the request, -1 for a root), or the
     nodes of ``mask`` [n] (int64 bit masks), or nodes 0..i (neither given: a chain; one node
     is plain decode). ``sel_in`` [n, k] int32 (with counts ``sel_n_in`` [n]) narrows each
@@ -193,17 +212,10 @@ def mla_tree_attn(cfg: AttnCfg, kv: PagedKV, q_abs: torch.Tensor, ctx_len: torch
         raise ValueError(f"block_table must have {B} rows")
     if out_dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("out_dtype must be float32 or bfloat16")
-    if parent is not None and mask is not None:
-        raise ValueError("give parent or mask, not both")
     if sel_in is None and sel_n_in is not None:
         raise ValueError("sel_n_in needs sel_in")
     q_abs = q_abs.contiguous()
-    m = None
-    if mask is not None:
-        if mask.dtype != torch.int64 or mask.device != dev or not mask.is_contiguous() or mask.numel() < n:
-            raise ValueError(f"mask must be a contiguous int64 tensor of {n} elements on {dev}")
-        m = mask.data_ptr()
-    par = None if parent is None else _i32(parent, "parent", dev, n)
+    par, m = _trees(parent, mask, n, dev)
     mode, sel, seln, stride, k = _lib.WL_MODE_DENSE, None, None, 0, 0
     if sel_in is not None:
         if sel_in.dim() != 2 or sel_in.shape[0] < n or sel_in.shape[1] < 1 or (sel_in.shape[1] > 1 and sel_in.stride(1) != 1):
