@@ -439,9 +439,9 @@ typedef struct wl_paged_kv {
  * whose pages do not all fit (then neither do those of later requests that
  * need any), or that would not fit its table row, gets none: short_out[b] is the
  * number of pages it lacks (0 = served), its slots are -1, and so are the table
- * entries of those pages (an attention or a commit over them sets the error word
- * and leaves them out; the caller drops the request's tokens, or frees pages and
- * plans again). Lengths below 0
+ * entries of those pages (an attention over them sets the error word and leaves
+ * their keys out, a commit sets it and commits nothing of the request; the caller
+ * drops the request's tokens, or frees pages and plans again). Lengths below 0
  * set the device error word; such a request gets short_out[b] = -1, no pages
  * and no tokens. Tokens are laid out request after request: token i of
  * request b is row cu_new[b] + i. Rows behind the last token (a padded batch)
@@ -543,8 +543,9 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
  * ctx_out must not be ctx_len. `latent` and `index` are host arrays of n_layers
  * pools that share the block table; `index` may be NULL, and an entry without
  * keys is skipped (a layer that owns no indexer). A parent that is not an
- * earlier node is never followed. Bad lengths or pages set the device error
- * word; the request's (the page's) rows then stay. */
+ * earlier node is never followed. A request of bad lengths, or with a page outside
+ * the pool under any of its nodes, sets the device error word and commits
+ * nothing: n_accept 0, next -1, ctx_out = ctx_len, its rows stay. */
 typedef struct wl_tree_commit_io {
     int32_t batch;
     int32_t n_nodes;

@@ -1,11 +1,14 @@
 """Positions of drafted trees in a plan, and whole steps with rotated keys, on the GPU. Everything here is
 compared bit for bit: whole numbers, and rows that the plain append writes at the same positions."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
 from oracle import paged_ref as R
 from test_gpu_paged import SCALE, T_MAX, bad_word, clean_device_error, cpu, i32  # noqa: F401
+from windlass_b200 import _lib
 from windlass_b200 import attn as A
 from windlass_b200 import paged as P
 
@@ -155,3 +158,34 @@ def test_branched_steps_leave_what_appending_the_accepted_tokens_leaves(by):
             assert torch.equal(ikeys.scale[slots], fkeys[b].scale[0, :len(pos)])
         ctx_len.copy_(done["ctx_len"])
     assert jumped >= 2  # the paths left the line
+
+
+@pytest.mark.parametrize("layers", [0, 1])
+def test_nothing_of_a_request_without_pages_is_committed(layers):
+    """Chains, whose accepted nodes stand where they belong already, and a jumping path. Request 0 has its pages; 1 lacks its
+    second page, 2 all of them, and 3's table row is too narrow; the drafts of 1 begin in a page that it holds."""
+    page = 8
+    pool = torch.randn(8 * page, 576, device="cuda", dtype=torch.bfloat16)
+    was = pool.clone()
+    ctx, new = [6, 5, 8, 20], [2, 5, 4, 6]
+    table, held = i32([[0, 9, 9], [1, 0, 0], [2, 0, 0], [3, 4, 5]]), i32([1, 1, 1, 3])
+    plan = P.page_plan(i32(ctx), i32(new), table, held, i32([7] * 8), i32([0]), page, 17)
+    assert cpu(plan["short"]).tolist() == [0, 1, 1, 1]
+    parent = i32([-1, 0] + [-1, 0, 0, 0, 2] + [-1, 0, 1, 2] + [-1, 0, 1, 2, 3, 4])
+    draft, target = i32([1] * 17), i32([1] * 17)
+    draft[3], draft[4] = 2, 1  # request 1 jumps from node 0 to node 2
+    ctx_len = i32(ctx)
+    if layers:
+        got = P.tree_commit(P.LayerCaches([P.PagedKV.packed(pool, page, table)]), ctx_len, plan["cu"], parent, draft, target)
+    else:  # the walk alone
+        out = {k: torch.full(s, 77, dtype=torch.int32, device="cuda") for k, s in
+               dict(n_accept=(4,), path=(4, 64), next=(4,), ctx_len=(4,)).items()}
+        io = _lib.TreeCommitIO(4, 17, ctx_len.data_ptr(), plan["cu"].data_ptr(), parent.data_ptr(), draft.data_ptr(), target.data_ptr(),
+                               page, 8, table.data_ptr(), 3, 3, 0, None, None, out["n_accept"].data_ptr(), out["path"].data_ptr(),
+                               out["next"].data_ptr(), out["ctx_len"].data_ptr())
+        assert _lib.lib().wl_tree_commit(C.byref(A.glm52_cfg(64)), C.byref(io), torch.cuda.current_stream().cuda_stream) == _lib.WL_OK
+        got = out
+    bad_word()
+    assert cpu(got["n_accept"]).tolist() == [2, 0, 0, 0] and cpu(got["next"]).tolist() == [1, -1, -1, -1]
+    assert cpu(got["ctx_len"]).tolist() == [8, 5, 8, 20]
+    assert cpu(got["path"])[:, 0].tolist() == [0, -1, -1, -1] and torch.equal(pool, was)

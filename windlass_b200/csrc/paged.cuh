@@ -335,14 +335,21 @@ __global__ void __launch_bounds__(COMMIT_THREADS) tree_commit_kernel(const __gri
             if (lane == 0) set_error(ERRC_BOUNDS, 43);
             n = 0;
         }
-        int par[2], tok[2], tgt[2];
+        // The cache row of every drafted node, before the walk: a request without a page under one of them (a plan with too
+        // few pages leaves such) wrote nothing, so nothing of it is committed.
+        const int* row = p.table + (long long)b * p.table_stride;
+        int par[2], tok[2], tgt[2], slot[2];
+        bool bad = false;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int j = lane + 32 * k;
             par[k] = j < n ? p.parent[r0 + j] : -2;
             tok[k] = j < n ? p.draft[r0 + j] : 0;
             tgt[k] = j < n ? p.target[r0 + j] : 0;
+            slot[k] = j < n ? page_slot(row, p.page_size, p.n_pages, ctx + j, 43) : 0;
+            bad |= slot[k] < 0;
         }
+        if (__any_sync(0xffffffffu, bad)) n = 0;
         int cur = 0, cnt = 0, want = -1, mine[2] = {-1, -1};
         while (cnt < n) {
             if (lane == (cnt & 31)) mine[cnt >> 5] = cur;
@@ -358,13 +365,10 @@ __global__ void __launch_bounds__(COMMIT_THREADS) tree_commit_kernel(const __gri
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int d = lane + 32 * k;
-            int s = -1, t = -1;
-            if (p.n_layers > 0 && mine[k] > d) {  // a node already in place does not move
-                const int* row = p.table + (long long)b * p.table_stride;
-                s = page_slot(row, p.page_size, p.n_pages, ctx + mine[k], 43);
-                t = page_slot(row, p.page_size, p.n_pages, ctx + d, 43);
-                if (t < 0) s = -1;
-            }
+            const int from = mine[k] < 0 ? 0 : mine[k];
+            const int s0 = __shfl_sync(0xffffffffu, slot[0], from & 31), s1 = __shfl_sync(0xffffffffu, slot[1], from & 31);
+            // a node already in place does not move
+            const int s = mine[k] > d ? (from < 32 ? s0 : s1) : -1, t = slot[k];
             src_sh[d] = s;
             dst_sh[d] = t;
             if (write) p.path[(long long)b * TREE_MAX + d] = mine[k];

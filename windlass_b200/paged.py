@@ -292,7 +292,7 @@ def tree_commit(layers: LayerCaches, ctx_len: torch.Tensor, cu_nodes: torch.Tens
     lowest child whose ``draft`` token is the current node's ``target`` token; its cache
     rows move to positions ctx_len + d in every layer. Returns n_accept [batch], path
     [batch, 64] (-1 behind the path), next [batch] (the target of the last node) and
-    ctx_len [batch] after the commit."""
+    ctx_len [batch] after the commit. Nothing of a request that lacks a page is committed."""
     dev = ctx_len.device
     B, n = ctx_len.numel(), parent.numel()
     first = layers.kvs[0]
