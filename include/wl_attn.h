@@ -502,7 +502,9 @@ int wl_cache_append_paged(const wl_attn_cfg* cfg, const wl_cache_append_io* io, 
  * position named twice counts twice);
  * WL_MODE_DENSE takes every key it sees. Rows that see nothing get ctx = 0 and
  * lse = -inf; rows of no request (behind cu_nodes[batch]) are left as they are.
- * Keys that a row does not see never reach it, whatever their rows hold.
+ * Keys that a row does not see never reach it, whatever their rows hold. A seen
+ * row's NaN or infinity gives NaN as the formula does (0 x infinity is NaN); a
+ * row whose every score is -infinity counts as one that sees nothing.
  * A request whose numbers are out of range (more than 64 nodes, rows outside
  * [0, n_nodes), ctx_len + nodes above cfg->T_max or its table), and a table
  * entry outside the pool, set the device error word; the request's rows are

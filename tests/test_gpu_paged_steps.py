@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import paged_ref as R
-from test_gpu_paged import SCALE, T_MAX, bad_word, clean_device_error, cpu, i32  # noqa: F401
+from test_gpu_paged import SCALE, T_MAX, Trees, bad_word, clean_device_error, cpu, i32  # noqa: F401
 from windlass_b200 import _lib
 from windlass_b200 import attn as A
 from windlass_b200 import paged as P
@@ -189,3 +189,41 @@ def test_nothing_of_a_request_without_pages_is_committed(layers):
     assert cpu(got["n_accept"]).tolist() == [2, 0, 0, 0] and cpu(got["next"]).tolist() == [1, -1, -1, -1]
     assert cpu(got["ctx_len"]).tolist() == [8, 5, 8, 20]
     assert cpu(got["path"])[:, 0].tolist() == [0, -1, -1, -1] and torch.equal(pool, was)
+
+
+@pytest.mark.parametrize("ctx,nodes", [([70], [5]), ([70], [15]), ([0], [14]), ([64], [13]), ([3000, 5], [13, 12]), ([4096], [3]), ([4096], [13])])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinities_of_seen_rows_give_what_the_formula_gives(ctx, nodes, dtype):
+    """Drafted rows with an infinity in a latent column, or in a roped one, seen by some nodes: NaN where the formula has it,
+    whichever nodes share the work and however the keys are cut. (A row whose scores are all -infinity gives zeros.)"""
+    t = Trees(ctx, nodes, 16, seed=41)
+    rng = np.random.default_rng(41)
+    masks = []
+    for n in nodes:
+        for i in range(n):
+            masks.append(1 << i | int(rng.integers(0, 1 << n)) & int(rng.integers(0, 1 << n)))
+    for j, (col, v) in {1: (0, np.inf), 2: (77, -np.inf), 3: (300, np.inf), 4: (511, -np.inf)}.items():
+        p = t.ctx[0] + j
+        t.c_kv[int(t.table[0][p // 16]) * 16 + p % 16, col] = v
+    if nodes[0] > 6:
+        p = t.ctx[0] + 6
+        slot = int(t.table[0][p // 16]) * 16 + p % 16
+        t.k_rot[slot, 3], t.c_kv[slot, 200] = np.inf, np.inf  # two that may meet as infinity - infinity
+    got = t.call(parent=None, mask=signed(masks), out_dtype=dtype)
+    with np.errstate(invalid="ignore"):
+        ref, lse, spread = R.tree_attn(t.q.float().cpu().numpy(), t.rows(), t.ctx, t.cu, masks, t.table, 16, SCALE)
+        keys = [np.r_[:t.ctx[b], [t.ctx[b] + j for j in range(n) if masks[t.cu[b] + i] >> j & 1]].astype(int) for b, n in enumerate(nodes) for i in range(n)]
+    rows = t.rows().astype(np.float64)
+    for r, k in enumerate(keys):
+        b = int(np.searchsorted(t.cu, r, "right")) - 1
+        with np.errstate(invalid="ignore"):
+            z = t.q[r].double().cpu().numpy() @ rows[t.table[b][k // 16].astype(int) * 16 + k % 16].T
+        none = (z == -np.inf).all(1)
+        ref[r][none], lse[r][none], spread[r][none] = 0, -np.inf, 0
+    o, z = got["ctx"].double().cpu().numpy(), got["lse"].double().cpu().numpy()
+    assert np.isnan(ref).any() and np.array_equal(np.isnan(o), np.isnan(ref))
+    assert np.array_equal(np.isnan(z), np.isnan(lse)) and np.array_equal(np.isneginf(z), np.isneginf(lse))
+    f, g = np.isfinite(ref), np.isfinite(lse)
+    spread = np.where(np.isfinite(spread), spread, 0)
+    tol = (2.0 ** -8 + 4e-4) * spread + (2.0 ** -8 * np.abs(ref) if dtype == torch.bfloat16 else 0)
+    assert np.all(np.abs(o - ref)[f] <= tol[f]) and np.abs(z - lse)[g].max(initial=0) < 4e-4

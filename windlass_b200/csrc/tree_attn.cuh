@@ -861,6 +861,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                 tc_fence_after();
                 const bool any = l_run != 0.f;  // (NaN counts: it reaches the result)
                 const float inv = any ? 1.f / l_run : 0.f;
+                const bool none = !any && out_part < 0;  // (a partial keeps the NaN of 0 x infinity)
                 const float lse = any ? (m_run + log2f(l_run)) * 0.69314718055994531f : -INFINITY;
                 if (!hi_half) {
                     if (out_part >= 0) p.lse_part[(long long)out_part * AT_H + h] = lse;
@@ -881,7 +882,7 @@ __global__ void __launch_bounds__(TaLayout<SEL>::THREADS, 1) tree_attn_kernel(co
                         float ov[32];
                         tmem_ld16x2_32<32>(tmem + lane_o + (uint32_t)(64 * c), ov);
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) ov[x] = any ? ov[x] * inv : 0.f;
+                        for (int x = 0; x < 32; ++x) ov[x] = none ? 0.f : ov[x] * inv;
                         if (narrow) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
@@ -1116,11 +1117,12 @@ __global__ void __launch_bounds__(TM_WARPS * 32) tree_merge_kernel(const TreePar
                 __syncthreads();  // the shared arrays are reused
                 if (wi > 0) continue;
             }
-            const float inv = W != 0.f ? 1.f / W : 0.f;  // (NaN counts: it reaches the result)
+            const float inv = 1.f / W;
             acc.x *= inv;
             acc.y *= inv;
             acc.z *= inv;
             acc.w *= inv;
+            if (W == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // (NaN does not count as none: it reaches the result)
             const long long at = ((long long)r * AT_H + h) * AT_DV + q * 128 + lane * 4;
             if (p.ctx_bf16) {
                 const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x, acc.y), c = __floats2bfloat162_rn(acc.z, acc.w);

@@ -26,8 +26,9 @@
 // Two nodes share V in one MMA: a drafted row that not both see, and that holds
 // a NaN or an infinity, would reach the other through 0 x NaN. In tiles with
 // drafted rows the value CTA therefore clears rows that neither sees and the
-// non-finite elements of rows that one sees (that node's own result is NaN
-// through its scores). Scores are per row; unseen ones are masked.
+// non-finite elements of rows that one sees. Whatever the weight p is (0, or NaN),
+// p x NaN and p x infinity are NaN there: the value CTA notes these columns for the
+// node that sees the row and writes NaN into them. Scores are per row; unseen ones are masked.
 #pragma once
 #include "tree_attn.cuh"
 
@@ -64,7 +65,8 @@ struct TpLayout {
     static constexpr uint32_t OFF_SUM = OFF_MAX + 1024;       // score CTA: one half's (sum, maximum) at an item's end [128]
     static constexpr uint32_t OFF_ITEM = OFF_SUM + 1024;      // item descriptors [2]
     static constexpr uint32_t OFF_LOST = OFF_ITEM + 128;      // keys lost to bad pages, per tile [8]
-    static constexpr uint32_t OFF_BAR = OFF_LOST + 64;
+    static constexpr uint32_t OFF_NAN = OFF_LOST + 64;        // value CTA: columns that are NaN, by item & 1 and node [2][2][512 bits]
+    static constexpr uint32_t OFF_BAR = OFF_NAN + 256;
     static constexpr int N_BARS = 34;
     static constexpr uint32_t OFF_MISC = OFF_BAR + N_BARS * 8;  // tensor-memory slot, longest, out count, slots [2][8]
     static constexpr uint32_t BYTES = OFF_MISC + 80 + 1024;
@@ -121,7 +123,10 @@ __device__ __forceinline__ void pair_load(const TreeMaps& tm, uint32_t dst, int 
     __syncwarp();
 }
 
-__device__ __forceinline__ uint32_t clear_nonfinite(uint32_t w) {  // two bf16
+__device__ __forceinline__ unsigned nonfinite(uint32_t w) {  // which of two bf16
+    return ((w & 0x7f80u) == 0x7f80u ? 1u : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 2u : 0u);
+}
+__device__ __forceinline__ uint32_t clear_nonfinite(uint32_t w) {
     if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
     if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
     return w;
@@ -138,6 +143,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
     float2* sum_sh = reinterpret_cast<float2*>(smem + L::OFF_SUM);
     TpItem* item_sh = reinterpret_cast<TpItem*>(smem + L::OFF_ITEM);
     unsigned long long* lost_sh = reinterpret_cast<unsigned long long*>(smem + L::OFF_LOST);
+    unsigned* nan_sh = reinterpret_cast<unsigned*>(smem + L::OFF_NAN);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
     uint64_t *ifull = bars, *ifree = bars + 2;  // item descriptors
     // score CTA
@@ -191,6 +197,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
         if (!score)
             for (int i = 0; i < TP_P; ++i) mbar_expect_tx(pfull + i, L::P + 512);
     }
+    if (tid < 64) nan_sh[tid] = 0;
     if (warp == TP_MMA_WARP) tmem_alloc(tmem_slot, 512);
     if (warp == TP_LOAD_WARP && lane < 3)
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &tm.q : lane == 1 ? &tm.ckv : &tm.krot)) : "memory");
@@ -554,7 +561,12 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                             uint4 w = make_uint4(0, 0, 0, 0);
                             if (one) {
                                 w = lds_v4(at);
-                                w = make_uint4(clear_nonfinite(w.x), clear_nonfinite(w.y), clear_nonfinite(w.z), clear_nonfinite(w.w));
+                                const unsigned gone = nonfinite(w.x) | nonfinite(w.y) << 2 | nonfinite(w.z) << 4 | nonfinite(w.w) << 6;
+                                if (gone) {  // columns 8 seg + .. of this chunk of 64 (128B swizzle)
+                                    const int seg = (lane ^ j) & 7, node = (m0 >> j) & 1 ? 0 : 1;
+                                    atomicOr(nan_sh + 32 * (k & 1) + 16 * node + 8 * x + 2 * (lane >> 3) + (seg >> 2), gone << (8 * (seg & 3)));
+                                    w = make_uint4(clear_nonfinite(w.x), clear_nonfinite(w.y), clear_nonfinite(w.z), clear_nonfinite(w.w));
+                                }
                             }
                             sts_v4(at, w);
                         }
@@ -579,8 +591,10 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
             }
             if (!ok) break;
             if (!(ok = pv_done(gt - 1, 88) && mbar_wait_cluster(finfull, (uint32_t)k & 1u, 89))) break;
+            if (!(ok = mbar_wait_fast(pok + ((gt - 1) & 3), (uint32_t)((gt - 1) >> 2) & 1u, 93))) break;  // all four warps' nan_sh
             tc_fence_after();
             const float inv = fin_sh[r];
+            const bool none = inv == 0.f && t.part < 0;  // a sum of zero: nothing seen (a partial keeps its NaN)
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(dsmem_addr(finfree, 0));
             // O / l through the last tile's space, 128-byte pieces of this warp's 32 rows in four boxes of 4 KB
@@ -602,8 +616,13 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                     }
                     __syncwarp();
                 }
+                const unsigned n0 = nan_sh[32 * (k & 1) + 16 * half + 2 * c], n1 = nan_sh[32 * (k & 1) + 16 * half + 2 * c + 1];
+                if (n0 | n1) {
 #pragma unroll
-                for (int x = 0; x < 64; ++x) o[x] *= inv;
+                    for (int x = 0; x < 64; ++x) o[x] = ((x < 32 ? n0 : n1) >> (x & 31)) & 1 ? __int_as_float(0x7fffffff) : o[x];
+                }
+#pragma unroll
+                for (int x = 0; x < 64; ++x) o[x] = none ? 0.f : o[x] * inv;
                 if (narrow) {
 #pragma unroll
                     for (int s = 0; s < 8; ++s) {
@@ -640,6 +659,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tree_pair_kernel(const TreePara
                 __threadfence_block();
                 if (atomicAdd(out_done, 1) == 3) {  // the last of the four warps gives the space back
                     *out_done = 0;
+                    for (int x = 0; x < 32; ++x) nan_sh[32 * (k & 1) + x] = 0;  // next used two items on
                     mbar_arrive(vfree + v);
                     mbar_arrive(vfree + v + 1);
                 }
