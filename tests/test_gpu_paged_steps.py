@@ -227,3 +227,12 @@ def test_infinities_of_seen_rows_give_what_the_formula_gives(ctx, nodes, dtype):
     spread = np.where(np.isfinite(spread), spread, 0)
     tol = (2.0 ** -8 + 4e-4) * spread + (2.0 ** -8 * np.abs(ref) if dtype == torch.bfloat16 else 0)
     assert np.all(np.abs(o - ref)[f] <= tol[f]) and np.abs(z - lse)[g].max(initial=0) < 4e-4
+
+
+def test_the_fields_of_a_paged_cache_do_not_change():
+    """Its addresses are taken once: a field that could be replaced would leave them behind."""
+    kv = P.PagedKV.packed(torch.zeros(32, 576, dtype=torch.bfloat16, device="cuda"), 16, i32([[0, 1]]))
+    for name in ("c_kv", "k_rot", "page_size", "block_table", "n_pages"):
+        with pytest.raises(AttributeError):
+            setattr(kv, name, getattr(kv, name))
+    assert kv.n_pages == 2 and kv.c().max_pages == 2

@@ -79,13 +79,13 @@ def _call(dev: torch.device, fn, *args) -> int:
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class PagedKV:
     """One layer's latent pool: c_kv [slots, 512] and k_rot [slots, 64] bf16 (rows of any
     stride that keeps them 16-byte aligned), pages of ``page_size`` rows (a multiple of
     8), ``block_table`` [batch, max_pages] int32. Slots past the last whole page are
-    not used. ``packed(kv)`` splits a [slots, 576] tensor. The views are taken when
-    the object is made; their contents, the table's included, may change freely. A table no
+    not used. ``packed(kv)`` splits a [slots, 576] tensor. The tensors' contents, the table's
+    included, may change freely, the tensors themselves not (other ones: a new object). A table no
     wider than the requests need lets ``mla_tree_attn`` choose its kernel well."""
     c_kv: torch.Tensor
     k_rot: torch.Tensor
@@ -104,11 +104,13 @@ class PagedKV:
             raise ValueError("c_kv and k_rot must be [slots, 512] and [slots, 64]")
         if krt.device != ckv.device:
             raise ValueError(f"k_rot must be on {ckv.device}, got {krt.device}")
-        self.n_pages = ckv.shape[0] // self.page_size if self.page_size > 0 else 0
-        if self.page_size <= 0 or self.page_size % 8 or self.n_pages <= 0:
+        n_pages = ckv.shape[0] // self.page_size if self.page_size > 0 else 0
+        if self.page_size <= 0 or self.page_size % 8 or n_pages <= 0:
             raise ValueError("page_size must be a multiple of 8 that the pool holds at least once")
         lat = LatentKV(ckv.unsqueeze(0), krt.unsqueeze(0)).c()
-        self._c = PagedKVC(lat, self.page_size, self.n_pages, *_table(t, t.shape[0], ckv.device))
+        # the addresses are taken here, so the fields are frozen
+        object.__setattr__(self, "n_pages", n_pages)
+        object.__setattr__(self, "_c", PagedKVC(lat, self.page_size, n_pages, *_table(t, t.shape[0], ckv.device)))
 
     def c(self) -> PagedKVC:
         return self._c
