@@ -544,7 +544,8 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
  * target[last node] (-1 without nodes), ctx_out[b] = ctx_len[b] + n_accept[b].
  * ctx_out must not be ctx_len. `latent` and `index` are host arrays of n_layers
  * pools that share the block table; `index` may be NULL, and an entry without
- * keys is skipped (a layer that owns no indexer). A parent that is not an
+ * keys is skipped (a layer that owns no indexer). No pool stands there twice
+ * (WL_ERR_ARG): its rows would move twice. A parent that is not an
  * earlier node is never followed. A request of bad lengths, or with a page outside
  * the pool under any of its nodes, sets the device error word and commits
  * nothing: n_accept 0, next -1, ctx_out = ctx_len, its rows stay. */

@@ -236,3 +236,15 @@ def test_the_fields_of_a_paged_cache_do_not_change():
         with pytest.raises(AttributeError):
             setattr(kv, name, getattr(kv, name))
     assert kv.n_pages == 2 and kv.c().max_pages == 2
+
+
+def test_layers_of_one_commit_have_pools_of_their_own():
+    t = i32([[0, 1]])
+    a, b = (torch.zeros(16, 576, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    keys = A.IndexKeys(torch.zeros(16, 128, dtype=torch.uint8, device="cuda"), torch.zeros(16, device="cuda"))
+    ka, kb = P.PagedKV.packed(a, 8, t), P.PagedKV.packed(b, 8, t)
+    P.LayerCaches([ka, kb], [keys, None])
+    with pytest.raises(ValueError, match="share one latent pool"):
+        P.LayerCaches([ka, ka])
+    with pytest.raises(ValueError, match="share one index pool"):
+        P.LayerCaches([ka, kb], [keys, keys])

@@ -201,6 +201,25 @@ def test_page_plan_takes_the_trees_in_one_form():
         P.page_plan(z, z, z.view(4, 1), z, z, z, 8, 4, mask=z)
 
 
+def test_tree_commit_refuses_a_pool_named_twice():
+    two = dict(n_layers=2, batch=0, ctx_len=None)
+    commit = lambda **kw: lib().wl_tree_commit(C.byref(cfg()), C.byref(commit_io(**two, **kw)), None)  # noqa: E731
+    pools = (LatentCache * 2)(pool(), pool(c_kv=FAKE + 4096, k_rot=FAKE + 5120))
+    assert commit(latent=pools) == OK
+    assert commit(latent=(LatentCache * 2)(pool(), pool())) == ARG
+    keys = [IndexCache(FAKE + 8192 * i, 0, FAKE, 0) for i in (1, 2)]
+    assert commit(latent=pools, index=(IndexCache * 2)(*keys)) == OK
+    assert commit(latent=pools, index=(IndexCache * 2)(keys[0], IndexCache())) == OK
+    assert commit(latent=pools, index=(IndexCache * 2)(IndexCache(), IndexCache())) == OK
+    assert commit(latent=pools, index=(IndexCache * 2)(keys[0], keys[0])) == ARG
+    for n in (78, 512, 700):
+        many = [pool(c_kv=FAKE + 4096 * i) for i in range(n)]
+        io = commit_io(n_layers=n, batch=0, ctx_len=None, latent=(LatentCache * n)(*many))
+        assert lib().wl_tree_commit(C.byref(cfg()), C.byref(io), None) == OK
+        io.latent[n - 1] = many[n // 3]
+        assert lib().wl_tree_commit(C.byref(cfg()), C.byref(io), None) == ARG
+
+
 # ---- the restatement -------------------------------------------------------------------------
 
 def test_restated_plan_gives_every_position_its_own_slot():

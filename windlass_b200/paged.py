@@ -254,7 +254,8 @@ def _tree_workspace(batch: int, n: int) -> int:
 class LayerCaches:
     """The pools that ``tree_commit`` moves rows in: ``kvs`` one ``PagedKV`` per layer, ``keys``
     None or one ``IndexKeys`` (pools [slots, 128] / [slots]) or None per layer. All layers
-    share one block table and page size."""
+    share one block table and page size, and no two a pool (keys that several layers read are
+    named once, at their owner)."""
 
     def __init__(self, kvs: list[PagedKV], keys: list[IndexKeys | None] | None = None):
         if not kvs:
@@ -283,6 +284,9 @@ class LayerCaches:
                     raise ValueError("index pools must be [slots, 128] with scales [slots], on the layers' device")
                 rows = min(rows, k.keys.shape[0], k.scale.shape[0])
                 self._index[i] = k.c()
+        for what, at in (("latent", [kv.c_kv.data_ptr() for kv in kvs]), ("index", [k.keys.data_ptr() for k in keys or () if k is not None])):
+            if len(set(at)) < len(at):
+                raise ValueError(f"two layers share one {what} pool: its rows would move twice")
         self.n_pages = rows // first.page_size
         if self.n_pages <= 0:
             raise ValueError("a pool holds less than one page")
