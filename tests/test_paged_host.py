@@ -10,6 +10,7 @@ import torch
 
 from oracle import paged_ref as R
 from windlass_b200 import _lib
+from windlass_b200 import attn as A
 from windlass_b200 import paged as P
 from windlass_b200._lib import IndexCache, LatentCache, PagedKVC, lib
 
@@ -218,6 +219,31 @@ def test_tree_commit_refuses_a_pool_named_twice():
         assert lib().wl_tree_commit(C.byref(cfg()), C.byref(io), None) == OK
         io.latent[n - 1] = many[n // 3]
         assert lib().wl_tree_commit(C.byref(cfg()), C.byref(io), None) == ARG
+
+
+def test_paged_append_refuses_what_it_would_read_past():
+    """Sizes and devices are looked at before anything else (no CUDA tensor is needed to see them)."""
+    keys = A.IndexKeys(torch.zeros(16, 128, dtype=torch.uint8), torch.zeros(16))
+    good = dict(slot=torch.zeros(3, dtype=torch.int32), cos=torch.zeros(3, 32), sin=torch.zeros(3, 32), k_raw=torch.zeros(3, 128),
+                k_norm_w=torch.zeros(128, dtype=torch.bfloat16), k_norm_b=torch.zeros(128, dtype=torch.bfloat16))
+    call = lambda **kw: P.cache_append_paged(cfg(), keys=keys, **{**good, **kw})  # noqa: E731
+    with pytest.raises(ValueError, match="CUDA"):
+        call()
+    for name, t in good.items():
+        if name == "slot":
+            continue
+        with pytest.raises(ValueError, match=f"{name} must hold {t.numel()}"):
+            call(**{name: t[:-1]})
+    with pytest.raises(ValueError, match="kv_raw must hold 1728"):
+        call(kv_raw=torch.zeros(2, 576))
+    with pytest.raises(ValueError, match="kv_norm_w must hold 512"):
+        call(kv_norm_w=torch.zeros(511, dtype=torch.bfloat16))
+    for name, t in good.items():
+        with pytest.raises(ValueError, match=f"{name} must be on cpu"):
+            call(**{name: t.to("meta")})
+    keys.scale = keys.scale.to("meta")
+    with pytest.raises(ValueError, match="one device"):
+        call()
 
 
 # ---- the restatement -------------------------------------------------------------------------

@@ -171,19 +171,34 @@ def page_release(done: torch.Tensor, block_table: torch.Tensor, n_held: torch.Te
     check(_call(dev, lib().wl_page_release, *args), "wl_page_release")
 
 
+# ``cache_append``'s tensors: elements a token, or in all
+_APPEND = (("k_raw", 128, 0), ("k_norm_w", 0, 128), ("k_norm_b", 0, 128), ("kv_raw", D_QK, 0), ("kv_norm_w", 0, KV_LORA))
+
+
 def cache_append_paged(cfg: AttnCfg, slot: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
                        kv: PagedKV | None = None, keys: IndexKeys | None = None, **kw) -> None:
     """``cache_append`` into pools: token i goes to row ``slot[i]`` (``page_plan``'s slots), -1
     is skipped. ``keys`` is the owner layer's index pool (keys [slots, 128], scale
-    [slots]); the other arguments are ``cache_append``'s."""
+    [slots]); the other arguments are ``cache_append``'s, for every token of ``slot``, and all
+    are on the pools' device."""
     pools = ([kv.c_kv] if kv is not None else []) + ([keys.keys, keys.scale] if keys is not None else [])
     if not pools:
         raise ValueError("cache_append_paged needs kv or keys")
     if keys is not None and (keys.keys.dim() != 2 or keys.scale.dim() != 1):
         raise ValueError("index pools must be [slots, 128] with scales [slots]")
+    dev, n = pools[0].device, slot.numel()
+    for t in pools:
+        if t.device != dev:
+            raise ValueError(f"the pools must be on one device, got {dev} and {t.device}")
+    for name, t, numel in (("slot", slot, n), ("cos", cos, 32 * n), ("sin", sin, 32 * n),
+                           *((k, kw[k], w * n if w else m) for k, w, m in _APPEND if kw.get(k) is not None)):
+        if t.device != dev:
+            raise ValueError(f"{name} must be on {dev}, got {t.device}")
+        if t.numel() < numel:
+            raise ValueError(f"{name} must hold {numel} elements, got {t.numel()}")
     io, hold = cache_append_io(slot, cos, sin, kv=None if kv is None else kv.latent(), keys=keys, **kw)
     n_slots = min(t.shape[0] for t in pools)
-    check(_call(pools[0].device, lib().wl_cache_append_paged, C.byref(cfg), C.byref(io), n_slots), "wl_cache_append_paged")
+    check(_call(dev, lib().wl_cache_append_paged, C.byref(cfg), C.byref(io), n_slots), "wl_cache_append_paged")
 
 
 # ---- attention of drafted trees ------------------------------------------------------------------
