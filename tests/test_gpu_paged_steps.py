@@ -248,3 +248,16 @@ def test_layers_of_one_commit_have_pools_of_their_own():
         P.LayerCaches([ka, ka])
     with pytest.raises(ValueError, match="share one index pool"):
         P.LayerCaches([ka, kb], [keys, keys])
+
+
+def test_lists_that_share_memory_are_refused():
+    """Rows that overlap (one list for all nodes, a window that slides): with counts, the lists ended at the row stride."""
+    t = Trees([50], [3], 16, seed=51)
+    one = i32([list(range(20))])
+    slide = torch.as_strided(i32(range(40)), (3, 20), (5, 1))
+    for lst in (one.expand(3, 20), slide):
+        for kw in (dict(), dict(sel_n_in=i32([20, 20, 20]))):
+            with pytest.raises(ValueError, match="must not overlap"):
+                t.call(sel_in=lst, **kw)
+    got = t.call(sel_in=one.expand(3, 20).contiguous())
+    t.check(got, sel=[np.arange(20)] * 3)

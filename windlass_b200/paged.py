@@ -239,6 +239,8 @@ def mla_tree_attn(cfg: AttnCfg, kv: PagedKV, q_abs: torch.Tensor, ctx_len: torch
             raise ValueError(f"sel_in must be [{n}, k] with consecutive entries")
         if sel_in.dtype != _I32 or sel_in.device != dev:
             raise ValueError(f"sel_in must be {_I32} on {dev}")
+        if sel_in.shape[0] > 1 and sel_in.stride(0) < sel_in.shape[1]:
+            raise ValueError("the rows of sel_in must not overlap (an expanded list: one contiguous row a node)")
         mode, sel, k = _lib.WL_MODE_CONSUMER, sel_in.data_ptr(), sel_in.shape[1]
         stride = sel_in.stride(0) if sel_in.shape[0] > 1 else k
         seln = None if sel_n_in is None else _i32(sel_n_in, "sel_n_in", dev, n)
