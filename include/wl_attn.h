@@ -441,8 +441,8 @@ typedef struct wl_paged_kv {
  * number of pages it lacks (0 = served), its slots are -1, and so are the table
  * entries of those pages (an attention over them sets the error word and leaves
  * their keys out, a commit sets it and commits nothing of the request; the caller
- * drops the request's tokens, or frees pages and plans again). Lengths below 0
- * set the device error word; such a request gets short_out[b] = -1, no pages
+ * drops the request's tokens, or frees pages and plans again). Lengths below 0,
+ * or that end past 2^31 - 1, set the device error word; such a request gets short_out[b] = -1, no pages
  * and no tokens. Tokens are laid out request after request: token i of
  * request b is row cu_new[b] + i. Rows behind the last token (a padded batch)
  * get -1. More tokens than n_tokens set the error word; the rows that fit are

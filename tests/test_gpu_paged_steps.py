@@ -261,3 +261,24 @@ def test_lists_that_share_memory_are_refused():
                 t.call(sel_in=lst, **kw)
     got = t.call(sel_in=one.expand(3, 20).contiguous())
     t.check(got, sel=[np.arange(20)] * 3)
+
+
+def test_lengths_that_pass_31_bits_are_flagged():
+    """A table that could hold them, of one large page over and over."""
+    page, wide, end = 1 << 20, 2100, (1 << 31) - 3
+    pool = torch.zeros(page, 576, device="cuda", dtype=torch.bfloat16)
+    table = torch.zeros(1, wide, dtype=torch.int32, device="cuda")
+    plan = P.page_plan(i32([end]), i32([10]), table, i32([2047]), i32([0] * 8), i32([8]), page, 10)
+    bad_word()
+    assert cpu(plan["short"]).tolist() == [-1] and cpu(plan["cu"]).tolist() == [0, 0] and (cpu(plan["slot"]) == -1).all()
+    kv = P.PagedKV.packed(pool, page, table)
+    cu, parent, tok = i32([0, 10]), i32([-1] + [0] * 9), i32([1] * 10)
+    done = P.tree_commit(P.LayerCaches([kv]), i32([end]), cu, parent, tok, tok)
+    bad_word()
+    assert cpu(done["n_accept"]).tolist() == [0] and cpu(done["ctx_len"]).tolist() == [end]
+    for nodes in (10, 13):
+        ctx = torch.full((nodes, 64, 512), 7.0, device="cuda")
+        P.mla_tree_attn(A.glm52_cfg((1 << 31) - 1), kv, torch.zeros(nodes, 64, 576, device="cuda", dtype=torch.bfloat16),
+                        i32([end - nodes]), i32([0, nodes]), ctx=ctx)
+        bad_word()
+        assert (ctx == 7).all()

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanParams p) {
             ctx = p.ctx_len[b];
             fresh = p.n_new[b];
             held = p.held[b];
-            if (ctx < 0 || fresh < 0 || held < 0 || held > p.max_pages) {
+            if (ctx < 0 || fresh < 0 || held < 0 || held > p.max_pages || (long long)ctx + fresh > 0x7fffffff) {
                 set_error(ERRC_BOUNDS, 41);
                 lack = -1;
                 fresh = 0;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(COMMIT_THREADS) tree_commit_kernel(const __gri
         const int r0 = p.cu[b], r1 = p.cu[b + 1], ctx = p.ctx_len[b];
         int n = r1 - r0;
         if (r0 < 0 || r1 > p.n_nodes || n < 0 || n > TREE_MAX || ctx < 0 ||
-            (long long)ctx + n > (long long)p.max_pages * p.page_size) {
+            (long long)ctx + n > min((long long)p.max_pages * p.page_size, 0x7fffffffll)) {
             if (lane == 0) set_error(ERRC_BOUNDS, 43);
             n = 0;
         }

@@ -1459,7 +1459,7 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     p.max_pages = kv.max_pages;
     p.page_size = kv.page_size;
     p.n_pages = kv.n_pages;
-    p.T_max = cfg->T_max;
+    p.T_max = cfg->T_max < INT32_MAX - 1024 ? cfg->T_max : INT32_MAX - 1024;  // positions are counted in whole tiles
     p.c_kv = static_cast<const __nv_bfloat16*>(kv.latent.c_kv);
     p.k_rot = static_cast<const __nv_bfloat16*>(kv.latent.k_rot);
     p.ckv_row = kv.latent.c_kv_row_stride;

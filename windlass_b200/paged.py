@@ -261,7 +261,7 @@ def mla_tree_attn(cfg: AttnCfg, kv: PagedKV, q_abs: torch.Tensor, ctx_len: torch
     return dict(ctx=ctx, lse=lse)
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=1024)
 def _tree_workspace(batch: int, n: int) -> int:
     return max(1, lib().wl_tree_attn_workspace_bytes(C.byref(_default_cfg()), batch, n))
 
