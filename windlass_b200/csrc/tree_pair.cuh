@@ -21,8 +21,8 @@
 // Bound: shared-memory bandwidth. A score SM writes 72 KB of keys, reads them for the MMAs and
 // writes and sends 16 KB of P, a value SM likewise: 1,410 cycles at 128 bytes; 1,434
 // (1 request x 64 nodes x 30K) and 1,484 (9 x 16 x 16K) measured.
-// 394 nodes of 16 requests x 32K keys 1,080 us, 1,110 to 1,220 once the power cap brings the
-// clock down to 1.6 to 1.75 GHz (1.16 to 1.31 PFLOP/s); 92 nodes of 8 x 16K 148 to 154 us.
+// Under lasting load the power cap brings the clock down: 394 nodes of 16 requests x 32K keys
+// 1,240 us (1.14 PFLOP/s), 92 nodes of 8 x 16K 173 us; in the first calls after a rest 1,090 and 155 us.
 // Two nodes share V in one MMA: a drafted row that not both see, and that holds
 // a NaN or an infinity, would reach the other through 0 x NaN. In tiles with
 // drafted rows the value CTA therefore clears rows that neither sees and the
@@ -45,7 +45,7 @@ constexpr int TP_UNITS = 6;   // score CTA: [even, odd][3] thirds of a tile (64 
 constexpr int TP_HALVES = 4;  // value CTA: [even, odd][2] halves of a tile (64 keys x 256 columns)
 constexpr int TP_P = 4;       // value CTA: tiles of P (score CTA: on their way), tile & 3
 constexpr uint32_t TP_TM_S = 384;  // score columns in tensor memory (the queries take [0, 288))
-// (0.8 us a tile; see TA_PRICE. At these and at (6, .12, .2): 9 requests, 109 nodes x 9K 126 / 144 us, 12, 74 x 13K
+// (0.8 us a tile; see TA_PRICE. From a rest, at these and at (6, .12, .2): 9 requests, 109 nodes x 9K 126 / 144 us, 12, 74 x 13K
 // 121 / 128, 8, 92 x 16K 166 / 169; 20, 235 x 3K 95 / 92.)
 constexpr TreePrice TP_PRICE = {6.f, 0.03f, 0.06f};
 

@@ -1416,7 +1416,8 @@ int wl_tree_commit(const wl_attn_cfg* cfg, const wl_tree_commit_io* io, void* st
 }
 
 // Partials a call may write: the schedule keeps to four CTA rounds of them, or
-// two per node, and no node is cut into more than TA_MAX_SPLIT runs.
+// two per node, and no node is cut into more than TA_MAX_SPLIT runs. (148: a B200's SMs, so that the size does not depend
+// on the device that is current when it is asked for.)
 static int64_t tree_parts_max(int32_t n_nodes) {
     const int64_t most = (int64_t)n_nodes * wl::TA_MAX_SPLIT, room = 4 * 148 > 2 * (int64_t)n_nodes ? 4 * 148 : 2 * (int64_t)n_nodes;
     return most < room ? most : room;
@@ -1490,7 +1491,7 @@ int wl_mla_tree_attn(const wl_attn_cfg* cfg, const wl_tree_attn_io* io, void* wo
     // Two nodes of a request at a time, by CTA pairs, when there is enough to do; one at a time for small trees (a
     // lone or last odd node leaves half of a pair's rows empty), for few keys (the pair's start and end take 5 us
     // longer) and for lists (a list per node). The lengths are on the device, so the keys are counted as if every
-    // row's request filled its table row. One at a time / pairs, us:
+    // row's request filled its table row. One at a time / pairs, us from a rest (the longest take up to 15 % more under lasting load):
     //   by keys      64 nodes x 1K 31 / 36; 40 x 2K 31 / 33; 16 x 8K 37 / 38; 64 x 2.5K 48 / 47; 47 x 4K 44 / 45;
     //                40 x 5K 54 / 48; 21 x 10K 45 / 42; 16 x 14K 52 / 47; 32 x 8K 60 / 52; 12 x 60K 120 / 115;
     //                92 x 16K 190 / 150; 394 x 32K 1625 / 1080
